@@ -55,7 +55,8 @@ int prana_ctx_destroy(prana_ctx *ctx); /* idempotent on NULL */
 int prana_ctx_set_stream(prana_ctx *ctx, void *cuda_stream);
 /* Wait for the context's kernel-level calls; a bounded device wait that gave
  * up in one of them (including prana_attention_decode_noalloc on this device)
- * returns PRANA_E_TIMEOUT here, once, and the context stays usable. */
+ * returns PRANA_E_TIMEOUT here, once, and the context stays usable; so does
+ * PRANA_E_INVALID for a row or length that lay outside its cache. */
 int prana_ctx_synchronize(prana_ctx *ctx);
 /* the context's own stream (model-level work always runs there), for event timing */
 int prana_ctx_stream(prana_ctx *ctx, void **cuda_stream);
@@ -191,6 +192,68 @@ int prana_attention_verify(prana_ctx *ctx, const float *q, const uint16_t *k_cac
 /* attention (attention.rs:236-284): causal over f32 in-window K/V; q, k, v and out 16-byte aligned */
 int prana_attention(prana_ctx *ctx, const float *q, const float *k, const float *v, size_t seq, size_t n_heads,
                     size_t n_kv_heads, size_t head_dim, float *out);
+/* ---- cache rows by index, and attention over trees of drafted tokens ----
+ * No counterpart in the reference (its cache is f16, one sequence, and its
+ * draft a chain).  A prana_kv_rows describes one layer's K and V in device
+ * memory the caller owns: [positions, n_kv_heads, head_dim] with the given
+ * element strides (the last dimension is contiguous), as f16 or as int8 with
+ * one f32 scale per position and head, [positions, n_kv_heads] with strides of
+ * its own: value = q * scale.  head_dim is at most 256.  One such cache may hold
+ * the rows of many sequences; row indexes, starts, lengths, paths and masks are
+ * DEVICE arrays.  What they hold is checked on the device: a row or a sequence
+ * that does not fit is left out, and the next prana_ctx_synchronize returns
+ * PRANA_E_INVALID, once.  Calls never synchronize. */
+#define PRANA_KV_F16 0
+#define PRANA_KV_Q8 1
+typedef struct prana_kv_rows {
+  int32_t kind; /* PRANA_KV_F16 or PRANA_KV_Q8 */
+  void *k, *v;
+  float *k_scale, *v_scale; /* PRANA_KV_Q8 only */
+  size_t positions, n_kv_heads, head_dim;
+  size_t row_stride, head_stride;
+  size_t scale_row_stride, scale_head_stride;
+} prana_kv_rows;
+/* Row rows[i] of the cache = row i of k and v ([n, n_kv_heads * head_dim], F32 or
+ * F16, src_stride elements from row to row), for rows[i] >= 0 (a negative index
+ * skips the row; an index named twice gets one of its rows).  An int8 cache
+ * quantises each head row as quantize_q8 does a block (matmul.rs:61-84): scale =
+ * amax / 127 (1 when amax is 0), round half away from zero, NaN to 0; a row
+ * holding an infinity gets an infinite scale and reads back as NaN.  An f16
+ * cache rounds to nearest. */
+int prana_kv_rows_write(prana_ctx *ctx, const prana_kv_rows *cache, const int32_t *rows, size_t n, int src_type,
+                        const void *k, const void *v, size_t src_stride);
+/* The values of rows rows[i] as dense F32 or F16 [n, n_kv_heads * head_dim]; zeros
+ * for a negative index. */
+int prana_kv_rows_read(prana_ctx *ctx, const prana_kv_rows *cache, const int32_t *rows, size_t n, int dst_type, void *k,
+                       void *v);
+/* After a tree was verified: for every sequence b and i < counts[b], row
+ * starts[b] + lens[b] + i becomes what row starts[b] + lens[b] + path[b][i] was
+ * (all of a sequence's rows move at once).  path is [n_seq, path_stride], at
+ * most 64 nodes wide. */
+int prana_kv_rows_move(prana_ctx *ctx, const prana_kv_rows *cache, const int32_t *starts, const int32_t *lens,
+                       const int32_t *path, const int32_t *counts, size_t n_seq, size_t path_stride);
+/* Attention of drafted nodes: sequence b has nodes node_offsets[b] ..
+ * node_offsets[b + 1] (rows of q and out, [n_nodes, n_heads * head_dim] f32; at
+ * most max_nodes <= 64 of them), lens[b] context rows from row starts[b] that all
+ * of its nodes see, and node j's own K / V in row starts[b] + lens[b] + j.  Bit j
+ * of masks[node] says whether the node sees node j of its sequence (itself
+ * included); masks NULL: node i sees nodes 0..i (a chain: attention_verify,
+ * attention.rs:296-333, for many sequences; with one node each,
+ * attention_decode, attention.rs:129-160).  Scores are scaled by 1/sqrt(head_dim);
+ * a node that sees nothing gets zeros; what a node does not see has no effect
+ * on it, NaN included, while a NaN or infinity in what it does see may make its
+ * row NaN.
+ * workspace: NULL for the context's scratch (then calls on several streams must
+ * not overlap), or workspace_bytes of 256-byte aligned device memory, at least
+ * what prana_attention_tree_workspace says, not shared by overlapping calls;
+ * its contents do not matter.  With a workspace the call allocates nothing and
+ * can be captured into a graph. */
+int prana_attention_tree_workspace(prana_ctx *ctx, size_t n_seq, size_t max_nodes, size_t n_heads, size_t n_kv_heads,
+                                   size_t head_dim, size_t *bytes);
+int prana_attention_tree(prana_ctx *ctx, const float *q, const prana_kv_rows *cache, const int32_t *starts,
+                         const int32_t *lens, const int32_t *node_offsets, const uint64_t *masks, size_t n_seq,
+                         size_t n_nodes, size_t max_nodes, size_t n_heads, void *workspace, size_t workspace_bytes,
+                         float *out);
 /* first index of the row maximum (infer.rs:560-568, sampler.rs:40-48) */
 int prana_argmax(prana_ctx *ctx, const float *x, size_t rows, size_t n, uint32_t *out);
 

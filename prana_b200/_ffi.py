@@ -40,6 +40,18 @@ class ModelConfig(C.Structure):
     ]
 
 
+class KvRowsView(C.Structure):
+    """prana_kv_rows: one layer's K and V rows in device memory."""
+    _fields_ = [
+        ("kind", C.c_int32), ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("positions", C.c_size_t), ("n_kv_heads", C.c_size_t), ("head_dim", C.c_size_t),
+        ("row_stride", C.c_size_t), ("head_stride", C.c_size_t),
+        ("scale_row_stride", C.c_size_t), ("scale_head_stride", C.c_size_t),
+    ]
+
+
+KV_F16, KV_Q8 = 0, 1
+
 P = C.c_void_p
 SZ = C.c_size_t
 I = C.c_int
@@ -86,6 +98,11 @@ SIGNATURES = {
     "prana_attention_verify": [P, P, P, P, SZ, SZ, SZ, SZ, SZ, P],
     "prana_attention": [P, P, P, P, SZ, SZ, SZ, SZ, P],
     "prana_argmax": [P, P, SZ, SZ, P],
+    "prana_kv_rows_write": [P, P, P, SZ, I, P, P, SZ],
+    "prana_kv_rows_read": [P, P, P, SZ, I, P, P],
+    "prana_kv_rows_move": [P, P, P, P, P, P, SZ, SZ],
+    "prana_attention_tree_workspace": [P, SZ, SZ, SZ, SZ, SZ, C.POINTER(SZ)],
+    "prana_attention_tree": [P, P, P, P, P, P, P, SZ, SZ, SZ, SZ, P, SZ, P],
     "prana_model_load_gguf": [P, C.c_char_p, C.POINTER(P)],
     "prana_model_load_gguf_ex": [P, C.c_char_p, I, C.POINTER(P)],
     "prana_model_load_gguf_tp": [P, C.c_char_p, I, I, P, C.POINTER(P)],

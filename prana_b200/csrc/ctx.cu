@@ -8,6 +8,7 @@
 
 #include "comm.h"
 #include "host.h"
+#include "mbar.cuh"
 #include "sampler.h"
 
 namespace prana {
@@ -234,8 +235,8 @@ int prana_ctx_stream(prana_ctx* c, void** stream) {
   return PRANA_OK;
 }
 
-// Waits for the kernel-level calls on the context's stream, then reports a
-// bounded device wait that gave up in any of them (the context's own error
+// Waits for the kernel-level calls on the context's stream, then reports rows
+// or lengths outside a cache as PRANA_E_INVALID, and a bounded device wait that gave up in any of them (the context's own error
 // word, and the no-allocation attention word of this device) as
 // PRANA_E_TIMEOUT, clearing the word so the context stays usable.
 int prana_ctx_synchronize(prana_ctx* c) {
@@ -246,9 +247,10 @@ int prana_ctx_synchronize(prana_ctx* c) {
   PRANA_CK(cudaMemcpy(&e, c->err, sizeof(unsigned), cudaMemcpyDeviceToHost));
   if (e) PRANA_CK(cudaMemset(c->err, 0, sizeof(unsigned)));
   if (int rc = noalloc_take_error(c->device, &e2)) return rc;
-  if (e || e2)
+  if ((e & ERR_TIMEOUT) || e2)
     return fail(PRANA_E_TIMEOUT, "a bounded device-side wait expired in a kernel-level call (%s)",
                 e ? "context" : "no-allocation attention");
+  if (e & ERR_RANGE) return fail(PRANA_E_INVALID, "a kernel-level call was given a row or a length outside its cache");
   return PRANA_OK;
 }
 
@@ -598,6 +600,126 @@ int prana_attention(prana_ctx* c, const float* q, const float* k, const float* v
   cudaError_t e = launch_attn_prefill(a, c->stream);
   if (e == cudaErrorInvalidValue) return fail(PRANA_E_UNSUPPORTED, "attention: head_dim %zu not built", hd);
   PRANA_CK(e);
+  return PRANA_OK;
+}
+
+// A cache view the kernels can index: kind, pointers, sizes and strides.
+static int kv_rows_dev(const prana_kv_rows* r, KvRowsDev* d) {
+  NEED(r, "cache is null");
+  NEED(r->kind == PRANA_KV_F16 || r->kind == PRANA_KV_Q8, "cache kind %d is neither PRANA_KV_F16 nor PRANA_KV_Q8", r->kind);
+  NEED(r->k && r->v, "cache k or v is null");
+  NEED(r->kind == PRANA_KV_F16 || (r->k_scale && r->v_scale), "an int8 cache needs k_scale and v_scale");
+  NEED(r->positions > 0 && r->positions <= (size_t)INT32_MAX - 1024, "cache positions %zu out of range", r->positions);
+  NEED(r->n_kv_heads > 0 && r->n_kv_heads <= 4096, "n_kv_heads %zu out of range", r->n_kv_heads);
+  NEED(r->head_dim > 0 && r->head_dim <= 256, "head_dim %zu out of range (1..256)", r->head_dim);
+  NEED(r->positions == 1 || r->row_stride >= r->head_dim, "row_stride %zu is less than head_dim", r->row_stride);
+  NEED(r->n_kv_heads == 1 || r->head_stride >= r->head_dim, "head_stride %zu is less than head_dim", r->head_stride);
+  NEED(r->kind == PRANA_KV_Q8 || !((reinterpret_cast<uintptr_t>(r->k) | reinterpret_cast<uintptr_t>(r->v)) & 1),
+       "an f16 cache must be 2-byte aligned");
+  NEED(r->kind == PRANA_KV_F16 ||
+           !((reinterpret_cast<uintptr_t>(r->k_scale) | reinterpret_cast<uintptr_t>(r->v_scale)) & 3),
+       "cache scales must be 4-byte aligned");
+  *d = KvRowsDev{r->k, r->v, r->k_scale, r->v_scale, r->kind == PRANA_KV_Q8, (int)r->positions, (int)r->n_kv_heads,
+                 (int)r->head_dim, r->row_stride, r->head_stride, r->scale_row_stride, r->scale_head_stride};
+  return PRANA_OK;
+}
+static bool aligned_to(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+int prana_kv_rows_write(prana_ctx* c, const prana_kv_rows* cache, const int32_t* rows, size_t n, int src_type,
+                        const void* k, const void* v, size_t src_stride) {
+  NEED(c, "ctx is null");
+  KvRowsDev d;
+  if (int rc = kv_rows_dev(cache, &d)) return rc;
+  NEED(src_type == PRANA_TYPE_F32 || src_type == PRANA_TYPE_F16, "source type %d is neither F32 nor F16", src_type);
+  if (!n) return PRANA_OK;
+  NEED(rows && k && v, "null argument");
+  NEED(n <= (size_t)INT32_MAX / d.n_kv, "%zu rows are too many", n);
+  NEED(n == 1 || src_stride >= cache->n_kv_heads * cache->head_dim, "src_stride %zu is less than a row", src_stride);
+  const size_t esz = src_type == PRANA_TYPE_F16 ? 2 : 4;
+  NEED(aligned_to(k, esz) && aligned_to(v, esz) && aligned_to(rows, 4), "misaligned argument");
+  DevScope ds(c->device);
+  PRANA_CK(launch_kv_rows_write(d, rows, k, v, src_type == PRANA_TYPE_F16, src_stride, (int)n, c->err, c->stream));
+  return PRANA_OK;
+}
+
+int prana_kv_rows_read(prana_ctx* c, const prana_kv_rows* cache, const int32_t* rows, size_t n, int dst_type, void* k,
+                       void* v) {
+  NEED(c, "ctx is null");
+  KvRowsDev d;
+  if (int rc = kv_rows_dev(cache, &d)) return rc;
+  NEED(dst_type == PRANA_TYPE_F32 || dst_type == PRANA_TYPE_F16, "destination type %d is neither F32 nor F16", dst_type);
+  if (!n) return PRANA_OK;
+  NEED(rows && k && v, "null argument");
+  NEED(n <= (size_t)INT32_MAX / d.n_kv, "%zu rows are too many", n);
+  const size_t esz = dst_type == PRANA_TYPE_F16 ? 2 : 4;
+  NEED(aligned_to(k, esz) && aligned_to(v, esz) && aligned_to(rows, 4), "misaligned argument");
+  DevScope ds(c->device);
+  PRANA_CK(launch_kv_rows_read(d, rows, k, v, dst_type == PRANA_TYPE_F16, (int)n, c->err, c->stream));
+  return PRANA_OK;
+}
+
+int prana_kv_rows_move(prana_ctx* c, const prana_kv_rows* cache, const int32_t* starts, const int32_t* lens,
+                       const int32_t* path, const int32_t* counts, size_t n_seq, size_t path_stride) {
+  NEED(c, "ctx is null");
+  KvRowsDev d;
+  if (int rc = kv_rows_dev(cache, &d)) return rc;
+  if (!n_seq || !path_stride) return PRANA_OK;
+  NEED(starts && lens && path && counts, "null argument");
+  NEED(n_seq <= (size_t)INT32_MAX, "%zu sequences are too many", n_seq);
+  NEED(path_stride <= (size_t)TREE_MAX_NODES, "a path of %zu nodes exceeds %d", path_stride, TREE_MAX_NODES);
+  NEED(aligned_to(starts, 4) && aligned_to(lens, 4) && aligned_to(path, 4) && aligned_to(counts, 4), "misaligned argument");
+  DevScope ds(c->device);
+  PRANA_CK(launch_kv_rows_move(d, starts, lens, path, counts, (int)n_seq, (int)path_stride, c->err, c->stream));
+  return PRANA_OK;
+}
+
+int prana_attention_tree_workspace(prana_ctx* c, size_t n_seq, size_t max_nodes, size_t n_heads, size_t n_kv_heads,
+                                   size_t head_dim, size_t* bytes) {
+  NEED(c && bytes, "null argument");
+  NEED(n_kv_heads > 0 && n_heads > 0 && n_heads % n_kv_heads == 0, "n_heads must be a multiple of n_kv_heads");
+  NEED(max_nodes <= (size_t)TREE_MAX_NODES, "%zu nodes per sequence exceed %d", max_nodes, TREE_MAX_NODES);
+  NEED(n_heads <= 65535 && head_dim <= 256 && n_seq <= (size_t)INT32_MAX, "sizes out of range");
+  *bytes = tree_workspace_bytes((int)n_seq, (int)max_nodes, (int)n_heads, (int)n_kv_heads, (int)head_dim, c->sm_count);
+  return PRANA_OK;
+}
+
+int prana_attention_tree(prana_ctx* c, const float* q, const prana_kv_rows* cache, const int32_t* starts,
+                         const int32_t* lens, const int32_t* node_offsets, const uint64_t* masks, size_t n_seq,
+                         size_t n_nodes, size_t max_nodes, size_t n_heads, void* workspace, size_t workspace_bytes,
+                         float* out) {
+  NEED(c, "ctx is null");
+  TreeArgs a{};
+  if (int rc = kv_rows_dev(cache, &a.c)) return rc;
+  NEED(n_heads > 0 && n_heads <= 65535 && n_heads % cache->n_kv_heads == 0, "n_heads must be a multiple of n_kv_heads");
+  NEED(max_nodes <= (size_t)TREE_MAX_NODES, "%zu nodes per sequence exceed %d", max_nodes, TREE_MAX_NODES);
+  if (!n_seq || !n_nodes || !max_nodes) return PRANA_OK;
+  NEED(q && starts && lens && node_offsets && out, "null argument");
+  NEED(n_seq <= (size_t)INT32_MAX && n_nodes <= (size_t)INT32_MAX, "too many sequences or nodes");
+  NEED(aligned_to(q, 4) && aligned_to(out, 4) && aligned_to(starts, 4) && aligned_to(lens, 4) &&
+           aligned_to(node_offsets, 4) && aligned_to(masks, 8),
+       "misaligned argument");
+  DevScope ds(c->device);
+  const size_t need = tree_workspace_bytes((int)n_seq, (int)max_nodes, (int)n_heads, a.c.n_kv, a.c.hd, c->sm_count);
+  if (workspace) {
+    NEED(workspace_bytes >= need, "the workspace has %zu bytes; %zu are needed", workspace_bytes, need);
+    NEED(aligned_to(workspace, 256), "the workspace must be 256-byte aligned");
+    a.work = workspace;
+  } else if (int rc = ctx_scratch(c, need, &a.work)) {
+    return rc;
+  }
+  a.q = q;
+  a.starts = starts;
+  a.lens = lens;
+  a.offsets = node_offsets;
+  a.masks = reinterpret_cast<const unsigned long long*>(masks);
+  a.n_seq = (int)n_seq;
+  a.n_nodes = (int)n_nodes;
+  a.max_nodes = (int)max_nodes;
+  a.n_heads = (int)n_heads;
+  a.out = out;
+  a.err = c->err;
+  a.sm_count = c->sm_count;
+  PRANA_CK(launch_attn_tree(a, c->stream));
   return PRANA_OK;
 }
 

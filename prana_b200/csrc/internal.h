@@ -198,6 +198,41 @@ cudaError_t launch_wait_never(unsigned polls, unsigned* err, cudaStream_t st);
 // first maximum over ranks: all = [world][16] (8 best values, then 8 index bit patterns)
 cudaError_t launch_tp_argmax(const float* all, int world, int m, uint32_t* tok_out, int* tok_next, cudaStream_t st);
 
+// ---------------------------------------------------------------- cache rows (rows.cu), tree attention (tree.cu)
+constexpr int TREE_MAX_NODES = 64;  // drafted nodes of one sequence: one mask bit each
+// K and V [positions][n_kv][hd], f16 or int8 with a scale per (position, head);
+// strides in elements
+struct KvRowsDev {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int q8;
+  int positions, n_kv, hd;
+  size_t row_stride, head_stride, scale_row, scale_head;
+};
+cudaError_t launch_kv_rows_write(const KvRowsDev& c, const int* rows, const void* k, const void* v, bool f16,
+                                 size_t src_stride, int n, unsigned* err, cudaStream_t st);
+cudaError_t launch_kv_rows_read(const KvRowsDev& c, const int* rows, void* k, void* v, bool f16, int n, unsigned* err,
+                                cudaStream_t st);
+cudaError_t launch_kv_rows_move(const KvRowsDev& c, const int* starts, const int* lens, const int* path,
+                                const int* counts, int n_seq, int path_stride, unsigned* err, cudaStream_t st);
+struct TreeArgs {
+  KvRowsDev c;
+  const float* q;  // [n_nodes][n_heads * hd]
+  const int* starts;
+  const int* lens;
+  const int* offsets;               // [n_seq + 1]
+  const unsigned long long* masks;  // [n_nodes]; null: a chain
+  int n_seq, n_nodes, max_nodes, n_heads;
+  float* out;  // [n_nodes][n_heads * hd]
+  void* work;
+  unsigned* err;
+  int sm_count;
+};
+size_t tree_workspace_bytes(int n_seq, int max_nodes, int n_heads, int n_kv, int hd, int sm_count);
+cudaError_t launch_attn_tree(const TreeArgs& a, cudaStream_t st);
+
 // ---------------------------------------------------------------- tensor-core GEMM (qgemm.cu)
 struct QgemmArgs {
   DevWeight w;

@@ -10,7 +10,8 @@
 
 namespace prana {
 
-enum : unsigned { ERR_NONE = 0, ERR_TIMEOUT = 1 };
+// bits of a device error word: a bounded wait ran out; a row or a length lay outside the cache
+enum : unsigned { ERR_NONE = 0, ERR_TIMEOUT = 1, ERR_RANGE = 2 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 

@@ -22,6 +22,7 @@ QK_K = 256
 BLOCK_BYTES = {TYPE_Q8_0: (32, 34), TYPE_Q4_0: (32, 18), TYPE_Q4_K: (256, 144), TYPE_Q6_K: (256, 210)}
 
 _ctxs: dict[int, C.c_void_p] = {}
+_tree_work: dict[tuple, int] = {}  # workspace bytes of attention_tree by sizes
 
 
 def context(device: int | None = None) -> C.c_void_p:
@@ -315,6 +316,170 @@ def attention(q, k, v, seq, n_heads, n_kv_heads, head_dim) -> torch.Tensor:
         raise ValueError("n_heads must be a multiple of n_kv_heads")
     out = torch.empty((seq, n_heads * head_dim), dtype=torch.float32, device=q.device)
     call("prana_attention", context(q.device.index), _ptr(q), _ptr(k), _ptr(v), seq, n_heads, n_kv_heads, head_dim, _ptr(out))
+    return out
+
+
+# ---- cache rows by index, and attention over trees of drafted tokens
+
+TREE_MAX_NODES = 64
+_SRC_TYPES = {torch.float32: TYPE_F32, torch.float16: TYPE_F16}
+
+
+class KvRows:
+    """One layer's K and V rows [positions, n_kv_heads, head_dim] in torch CUDA
+    memory: float16, or int8 with f32 scales [positions, n_kv_heads] (value =
+    q * scale).  Any strides, as long as the last dimension is contiguous and k
+    and v (and the two scales) are laid out alike.  The rows of many sequences
+    may share one KvRows."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "quantized", "_view")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None,
+                 v_scale: torch.Tensor | None = None):
+        shape, strides = k.shape, k.stride()
+        if len(shape) != 3 or v.shape != shape or v.stride() != strides or v.dtype != k.dtype:
+            raise ValueError("k and v must be [positions, n_kv_heads, head_dim] of one type and layout")
+        if strides[2] != 1 and shape[2] != 1:
+            raise ValueError("the head dimension must be contiguous")
+        device = k.device
+        if device.type != "cuda" or v.device != device:
+            raise ValueError("expected CUDA tensors of one device")
+        self.quantized = k.dtype == torch.int8
+        scale_strides = (0, 0)
+        if self.quantized:
+            if k_scale is None or v_scale is None:
+                raise ValueError("an int8 cache needs k_scale and v_scale")
+            scale_strides = k_scale.stride()
+            if k_scale.shape != shape[:2] or v_scale.shape != shape[:2] or v_scale.stride() != scale_strides:
+                raise ValueError("scales must be [positions, n_kv_heads] of one layout")
+            if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+                raise TypeError("scales must be float32")
+            if k_scale.device != device or v_scale.device != device:
+                raise ValueError("expected CUDA tensors of one device")
+        elif k.dtype != torch.float16:
+            raise TypeError("a cache holds float16 or int8")
+        elif k_scale is not None or v_scale is not None:
+            raise ValueError("a float16 cache has no scales")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._view = _ffi.KvRowsView(
+            _ffi.KV_Q8 if self.quantized else _ffi.KV_F16, k.data_ptr(), v.data_ptr(),
+            k_scale.data_ptr() if self.quantized else None, v_scale.data_ptr() if self.quantized else None,
+            shape[0], shape[1], shape[2], strides[0], strides[1], scale_strides[0], scale_strides[1])
+
+    @classmethod
+    def alloc(cls, positions: int, n_kv_heads: int, head_dim: int, quantized: bool = True,
+              device: int | str | torch.device = "cuda") -> "KvRows":
+        """A zeroed cache; scales lie head by head, so that one head's positions are adjacent."""
+        shape = (positions, n_kv_heads, head_dim)
+        dt = torch.int8 if quantized else torch.float16
+        k, v = torch.zeros(shape, dtype=dt, device=device), torch.zeros(shape, dtype=dt, device=device)
+        if not quantized:
+            return cls(k, v)
+        s = torch.zeros((2, n_kv_heads, positions), dtype=torch.float32, device=device)
+        return cls(k, v, s[0].t(), s[1].t())
+
+    def _int32(self, t: torch.Tensor, shape: tuple, what: str) -> int:
+        if t.dtype != torch.int32:
+            raise TypeError(f"{what} must be int32")
+        if t.shape != shape:
+            raise ValueError(f"{what} must have shape {list(shape)}")
+        if t.device != self.k.device or not t.is_contiguous():
+            raise ValueError(f"{what} must be a contiguous tensor on the cache's device")
+        return t.data_ptr()
+
+
+def kv_rows_write(cache: KvRows, rows: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
+    """Cache row rows[i] (int32; negative: skipped) = row i of k and v, [n, n_kv_heads,
+    head_dim] or [n, n_kv_heads * head_dim] in float32 or float16.  An int8 cache
+    quantises each head row as it is written: scale = amax / 127, as quantize_q8."""
+    view = cache._view
+    n, width = rows.numel(), view.n_kv_heads * view.head_dim
+    if k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.numel() != n * width:
+        raise ValueError("k and v must hold one cache row for each index, laid out alike")
+    if k.dtype not in _SRC_TYPES:
+        raise TypeError("k and v must be float32 or float16")
+    if k.device != cache.k.device or v.device != cache.k.device:
+        raise ValueError("k and v must be on the cache's device")
+    stride = k.stride(0) if n else 0
+    if n and not k[0].is_contiguous():
+        raise ValueError("a row of k and v must be contiguous")
+    call("prana_kv_rows_write", context(cache.k.device.index), C.byref(view), cache._int32(rows, (n,), "rows"), n,
+         _SRC_TYPES[k.dtype], k.data_ptr(), v.data_ptr(), stride)
+
+
+def kv_rows_read(cache: KvRows, rows: torch.Tensor, dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
+    """The values of cache rows rows[i] (zeros for a negative index), K and V as
+    [n, n_kv_heads, head_dim] in float32 or float16."""
+    if dtype not in _SRC_TYPES:
+        raise TypeError("rows are read as float32 or float16")
+    view, n = cache._view, rows.numel()
+    out = torch.empty((2, n, view.n_kv_heads, view.head_dim), dtype=dtype, device=cache.k.device)
+    k, v = out.unbind(0)
+    call("prana_kv_rows_read", context(cache.k.device.index), C.byref(view), cache._int32(rows, (n,), "rows"), n,
+         _SRC_TYPES[dtype], k.data_ptr(), v.data_ptr())
+    return k, v
+
+
+def kv_rows_move(cache: KvRows, starts: torch.Tensor, lens: torch.Tensor, path: torch.Tensor, counts: torch.Tensor) -> None:
+    """Close accepted branches up: for i < counts[b], row starts[b] + lens[b] + i becomes
+    what row starts[b] + lens[b] + path[b, i] was.  path is int32 [n_seq, at most 64]."""
+    n = starts.numel()
+    if path.dim() != 2:
+        raise ValueError("path must be [n_seq, nodes]")
+    call("prana_kv_rows_move", context(cache.k.device.index), C.byref(cache._view), cache._int32(starts, (n,), "starts"),
+         cache._int32(lens, (n,), "lens"), cache._int32(path, (n, path.shape[1]), "path"),
+         cache._int32(counts, (n,), "counts"), n, path.shape[1])
+
+
+def tree_masks(parents) -> list[int]:
+    """Masks of one tree from its nodes' parents (-1: the root's; a parent comes
+    before its children): each node sees its ancestors and itself.  As signed
+    64-bit values, for an int64 tensor."""
+    if len(parents) > TREE_MAX_NODES:
+        raise ValueError(f"a tree has at most {TREE_MAX_NODES} nodes")
+    masks: list[int] = []
+    for i, p in enumerate(parents):
+        if not -1 <= p < i:
+            raise ValueError(f"node {i} has parent {p}: a parent comes before its children")
+        masks.append((masks[p] if p >= 0 else 0) | 1 << i)
+    return [m - (1 << 64) if m >> 63 else m for m in masks]
+
+
+def attention_tree(q: torch.Tensor, cache: KvRows, starts: torch.Tensor, lens: torch.Tensor, offsets: torch.Tensor,
+                   max_nodes: int, n_heads: int, masks: torch.Tensor | None = None,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of drafted tokens: sequence b has nodes offsets[b] .. offsets[b + 1]
+    (rows of q and of the result, [n_nodes, n_heads * head_dim] f32, at most
+    max_nodes <= 64 each), lens[b] context rows from cache row starts[b], and node
+    j's K / V in row starts[b] + lens[b] + j.  Every node sees its context and the
+    nodes whose bits are set in its mask (int64 [n_nodes], see tree_masks; None:
+    itself and the nodes before it).  With one node per sequence this is
+    attention_decode for a batch.  starts, lens, offsets are int32."""
+    view, n_seq, n_nodes = cache._view, starts.numel(), q.shape[0]
+    device = cache.k.device
+    width = n_heads * view.head_dim
+    if q.dtype != torch.float32 or q.device != device or not q.is_contiguous() or q.numel() != n_nodes * width:
+        raise ValueError("q must be a contiguous float32 [n_nodes, n_heads * head_dim] on the cache's device")
+    mask_ptr = None
+    if masks is not None:
+        if masks.dtype != torch.int64 or masks.shape != (n_nodes,) or masks.device != device or not masks.is_contiguous():
+            raise ValueError("masks must be a contiguous int64 [n_nodes] on the cache's device")
+        mask_ptr = masks.data_ptr()
+    if out is None:
+        out = torch.empty((n_nodes, width), dtype=torch.float32, device=device)
+    elif out.dtype != torch.float32 or out.device != device or not out.is_contiguous() or out.numel() != n_nodes * width:
+        raise ValueError("out must be a contiguous float32 [n_nodes, n_heads * head_dim] on the cache's device")
+    ctx = context(device.index)
+    key = (device.index, n_seq, max_nodes, n_heads, view.n_kv_heads, view.head_dim)
+    size = _tree_work.get(key)
+    if size is None:
+        bytes_ = C.c_size_t()
+        call("prana_attention_tree_workspace", ctx, n_seq, max_nodes, n_heads, view.n_kv_heads, view.head_dim, C.byref(bytes_))
+        size = _tree_work[key] = bytes_.value
+    work = torch.empty(size, dtype=torch.uint8, device=device)  # of this stream: calls on other streams have their own
+    call("prana_attention_tree", ctx, q.data_ptr(), C.byref(view), cache._int32(starts, (n_seq,), "starts"),
+         cache._int32(lens, (n_seq,), "lens"), cache._int32(offsets, (n_seq + 1,), "offsets"), mask_ptr, n_seq, n_nodes,
+         max_nodes, n_heads, work.data_ptr(), size, out.data_ptr())
     return out
 
 
