@@ -248,8 +248,8 @@ int prana_kv_rows_move(prana_ctx *ctx, const prana_kv_rows *cache, const int32_t
  * what prana_attention_tree_workspace says, not shared by overlapping calls;
  * its contents do not matter.  With a workspace the call allocates nothing and
  * can be captured into a graph. */
-int prana_attention_tree_workspace(prana_ctx *ctx, size_t n_seq, size_t max_nodes, size_t n_heads, size_t n_kv_heads,
-                                   size_t head_dim, size_t *bytes);
+int prana_attention_tree_workspace(prana_ctx *ctx, size_t max_nodes, size_t n_heads, size_t n_kv_heads, size_t head_dim,
+                                   size_t *bytes);
 int prana_attention_tree(prana_ctx *ctx, const float *q, const prana_kv_rows *cache, const int32_t *starts,
                          const int32_t *lens, const int32_t *node_offsets, const uint64_t *masks, size_t n_seq,
                          size_t n_nodes, size_t max_nodes, size_t n_heads, void *workspace, size_t workspace_bytes,

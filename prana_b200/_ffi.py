@@ -101,7 +101,7 @@ SIGNATURES = {
     "prana_kv_rows_write": [P, P, P, SZ, I, P, P, SZ],
     "prana_kv_rows_read": [P, P, P, SZ, I, P, P],
     "prana_kv_rows_move": [P, P, P, P, P, P, SZ, SZ],
-    "prana_attention_tree_workspace": [P, SZ, SZ, SZ, SZ, SZ, C.POINTER(SZ)],
+    "prana_attention_tree_workspace": [P, SZ, SZ, SZ, SZ, C.POINTER(SZ)],
     "prana_attention_tree": [P, P, P, P, P, P, P, SZ, SZ, SZ, SZ, P, SZ, P],
     "prana_model_load_gguf": [P, C.c_char_p, C.POINTER(P)],
     "prana_model_load_gguf_ex": [P, C.c_char_p, I, C.POINTER(P)],

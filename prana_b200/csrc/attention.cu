@@ -841,14 +841,6 @@ struct AcSmem {
   static_assert(sizeof(float) * 8 * AM_ROWS * (HD + 2) <= 2 * STAGE, "warp merge buffer (both stages)");
 };
 
-__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
-      "[%5];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
-      : "memory");
-}
-
 // byte offset of the 16-byte chunk `chunk` (of 8 halves) of position row r in a
 // 128-byte-swizzled box
 __device__ __forceinline__ int swz(int r, int chunk) { return r * 128 + ((chunk ^ (r & 7)) << 4); }
@@ -1777,6 +1769,24 @@ static bool encode_cache_map(CUtensorMap* m, const __half* base, int positions, 
   return fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half*>(base), dims, strides, box, es,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// {hd, n_kv, positions} view of cache rows of any strides, `box` elements x 1
+// head x 128 positions; elements past hd and rows past `positions` read as 0
+bool encode_rows_map(CUtensorMap* m, const void* base, bool q8, int positions, int n_kv, int hd, size_t row_stride,
+                     size_t head_stride, int box) {
+  EncodeTiledFn fn = encode_tiled();
+  const size_t esz = q8 ? 1 : 2;
+  // a stride nothing steps over need not be one the tensor map takes
+  const size_t hs = n_kv == 1 ? 256 : head_stride * esz, rs = positions == 1 ? 256 : row_stride * esz;
+  if (!fn || ((reinterpret_cast<uintptr_t>(base) | hs | rs | hd * esz) & 15) || hs >> 40 || rs >> 40) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)n_kv, (cuuint64_t)positions};
+  const cuuint64_t strides[2] = {(cuuint64_t)hs, (cuuint64_t)rs};
+  const cuuint32_t boxes[3] = {(cuuint32_t)box, 1, 128};
+  const cuuint32_t es[3] = {1, 1, 1};
+  return fn(m, q8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims,
+            strides, boxes, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 void attn_make_maps(AttnArgs& a, int positions) {

@@ -673,13 +673,13 @@ int prana_kv_rows_move(prana_ctx* c, const prana_kv_rows* cache, const int32_t* 
   return PRANA_OK;
 }
 
-int prana_attention_tree_workspace(prana_ctx* c, size_t n_seq, size_t max_nodes, size_t n_heads, size_t n_kv_heads,
+int prana_attention_tree_workspace(prana_ctx* c, size_t max_nodes, size_t n_heads, size_t n_kv_heads,
                                    size_t head_dim, size_t* bytes) {
   NEED(c && bytes, "null argument");
   NEED(n_kv_heads > 0 && n_heads > 0 && n_heads % n_kv_heads == 0, "n_heads must be a multiple of n_kv_heads");
   NEED(max_nodes <= (size_t)TREE_MAX_NODES, "%zu nodes per sequence exceed %d", max_nodes, TREE_MAX_NODES);
-  NEED(n_heads <= 65535 && head_dim <= 256 && n_seq <= (size_t)INT32_MAX, "sizes out of range");
-  *bytes = tree_workspace_bytes((int)n_seq, (int)max_nodes, (int)n_heads, (int)n_kv_heads, (int)head_dim, c->sm_count);
+  NEED(n_heads <= 65535 && head_dim <= 256, "sizes out of range");
+  *bytes = tree_workspace_bytes((int)max_nodes, (int)n_heads, (int)n_kv_heads, (int)head_dim, c->sm_count);
   return PRANA_OK;
 }
 
@@ -691,6 +691,7 @@ int prana_attention_tree(prana_ctx* c, const float* q, const prana_kv_rows* cach
   TreeArgs a{};
   if (int rc = kv_rows_dev(cache, &a.c)) return rc;
   NEED(n_heads > 0 && n_heads <= 65535 && n_heads % cache->n_kv_heads == 0, "n_heads must be a multiple of n_kv_heads");
+  NEED(n_heads / cache->n_kv_heads <= 1024, "more than 1024 heads share a kv head");
   NEED(max_nodes <= (size_t)TREE_MAX_NODES, "%zu nodes per sequence exceed %d", max_nodes, TREE_MAX_NODES);
   if (!n_seq || !n_nodes || !max_nodes) return PRANA_OK;
   NEED(q && starts && lens && node_offsets && out, "null argument");
@@ -699,7 +700,7 @@ int prana_attention_tree(prana_ctx* c, const float* q, const prana_kv_rows* cach
            aligned_to(node_offsets, 4) && aligned_to(masks, 8),
        "misaligned argument");
   DevScope ds(c->device);
-  const size_t need = tree_workspace_bytes((int)n_seq, (int)max_nodes, (int)n_heads, a.c.n_kv, a.c.hd, c->sm_count);
+  const size_t need = tree_workspace_bytes((int)max_nodes, (int)n_heads, a.c.n_kv, a.c.hd, c->sm_count);
   if (workspace) {
     NEED(workspace_bytes >= need, "the workspace has %zu bytes; %zu are needed", workspace_bytes, need);
     NEED(aligned_to(workspace, 256), "the workspace must be 256-byte aligned");

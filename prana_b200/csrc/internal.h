@@ -230,7 +230,10 @@ struct TreeArgs {
   unsigned* err;
   int sm_count;
 };
-size_t tree_workspace_bytes(int n_seq, int max_nodes, int n_heads, int n_kv, int hd, int sm_count);
+// tensor map of cache rows (attention.cu); false: their strides or alignment do not take one
+bool encode_rows_map(CUtensorMap* m, const void* base, bool q8, int positions, int n_kv, int hd, size_t row_stride,
+                     size_t head_stride, int box);
+size_t tree_workspace_bytes(int max_nodes, int n_heads, int n_kv, int hd, int sm_count);
 cudaError_t launch_attn_tree(const TreeArgs& a, cudaStream_t st);
 
 // ---------------------------------------------------------------- tensor-core GEMM (qgemm.cu)

@@ -7,6 +7,7 @@
 // A place that a node does not see takes no part, whatever it holds.
 #include "internal.h"
 #include "mbar.cuh"
+#include "tc.cuh"
 
 namespace prana {
 
@@ -98,13 +99,1034 @@ __global__ void __launch_bounds__(TR_THREADS) tree_simple_kernel(const TreeArgs 
     if (tid + e * TR_THREADS < hd) a.out[row_q + tid + e * TR_THREADS] = l == 0.0f ? 0.0f : o[e] / l;
 }
 
-size_t tree_workspace_bytes(int, int, int, int, int, int) { return 256; }
+// ---------------------------------------------------------------- tcgen05
+// Head sizes up to 128 whose rows a tensor map can describe.  The (node, head)
+// pairs that share a kv head are columns; a unit of work is (sequence, kv head,
+// chunk of columns), its tiles are 128 positions each, and the tiles of all
+// units, in order, are dealt to the CTAs (one per SM) in equal contiguous
+// shares, so ragged batches stay balanced.  A unit inside one share is finished
+// there; otherwise its shares leave (max, sum, o) partials for tree_merge_kernel.
+//
+// Exactness.  An f16 cache: q and p enter as f16 head + remainder pairs (22
+// bits), K and V as they are.  An int8 cache: q and p as three signed base-256
+// digits (23 bits) and kind::i8 products, so K and V enter as they lie in memory
+// with no conversion, and every product and sum is an exact integer; a digit's
+// sum stays below 2^22 (128 x 128 x 128).  The K scale multiplies the score in
+// f32.  The V scale, 2^e * m, goes with the probability: e is added to the score
+// (in powers of two), so that p * 2^e of a tile is taken against its own largest
+// value, and m scales the digits.  The fixed point is then as fine as what the
+// tile adds to the output needs: against a running maximum of the scores alone,
+// 10^5 places of 2^-26 beside one large score with a small value would all round
+// to nothing.
+//
+// Roles (20 warps): 16 loads K and V tiles by TMA into a ring of slots, 17 issues
+// S = K . q^T (M = 128 positions), 18 issues O^T = V^T . p^T (M = dims; V is read
+// MN-major as it lies, p is written position by position), 19 prepares the next
+// segment's columns, and four groups of four warps do the softmax, a thread per
+// position for S and a thread per dim for O, 16 columns at most.  The groups form
+// teams with a tile each: up to 16 columns four teams of one group, with 32 two
+// teams of two, with 64 one team of four, whose columns share one product.  (A
+// product of few columns costs the 4 KB of its K or V rows, 40 cycles at 32
+// columns and 100 at 192: four of 48 took twice one of 192.)  The cache is so read
+// once for 64 columns.
+constexpr int TT_GROUPS = 4, TT_SOFT = TT_GROUPS * 128, TT_THREADS = TT_SOFT + 128;
+constexpr int TT_TMA_WARP = 16, TT_S_WARP = 17, TT_O_WARP = 18, TT_Q_WARP = 19;
+constexpr int TT_TILE = 128;
+constexpr int TT_MAX_SLOTS = 10;
+constexpr float TT_DIGITS = 8355711.0f;  // 0x7f7f7f: the largest value of three balanced digits
+constexpr float TT_BIAS = 8421504.0f;    // 2^23 + 0x8080: rounds to an integer whose bytes are the digits, two of them + 128
+constexpr float LOG2E = 1.4426950408889634f;
+
+// What a CTA leaves for the merge: the unit that began in it and went on in
+// the next n - 1 CTAs (n = 0: none).
+struct TreePart {
+  int n, cols, vh0, kvh, off, pad[3];
+};
+struct TreeTcArgs {
+  CUtensorMap tm_k, tm_v;
+  TreeArgs t;
+  int boxes;        // TMA boxes of a tile's K (or V): 1, or 2 for an f16 head above 64
+  int slots;        // ring slots
+  TreePart* parts;  // [CTAs]
+  float2* part_ml;  // [2 * CTAs][columns] (max, sum)
+  float* part_o;    // [2 * CTAs][columns][hd]
+};
+
+// NQ columns of a group, CG groups in a team
+template <bool Q8, int NQ, int CG>
+struct TtShape {
+  static constexpr int CH = NQ * CG;                               // columns of a CTA
+  static constexpr int TG = TT_GROUPS / CG;                        // teams: tiles in work at once
+  static constexpr int N = Q8 ? (NQ == 8 ? 32 : 3 * CH) : 2 * CH;  // MMA columns: digit by digit, or heads and remainders
+  static constexpr int CS = (N + 31) / 32 * 32;                    // TMEM columns between accumulators
+  static constexpr int TMEM = 2 * TG * CS <= 128 ? 128 : 2 * TG * CS <= 256 ? 256 : 512;
+  static constexpr int QSZ = N * (Q8 ? 128 : 256);                 // bytes of the q operand
+  static constexpr int BLOCKS = (N * (Q8 ? 1 : 2) + 63) / 64;      // 64-byte blocks of a p row
+  static constexpr int PBLOCK = TT_TILE * 64, PSZ = BLOCKS * PBLOCK;  // bytes of a block, of a team's p operand
+  static constexpr int RING = (CG < 4 ? 160 : Q8 ? 144 : 128) * 1024;
+  static constexpr int OFF_P = RING, OFF_Q = OFF_P + TG * PSZ;
+  static constexpr size_t BYTES = 1024 + OFF_Q + QSZ;
+  static_assert(2 * TG * CS <= 512, "TMEM");
+  static_assert(TG == 1 || PSZ >= CG * NQ * 128 * 4, "the groups' o pass through the p operand");
+};
+
+// instruction descriptors: M = 128; i8 (s32 accumulators) or f16 (f32); `mn`: both operands MN-major
+template <bool Q8>
+constexpr uint32_t tt_idesc(int n, bool mn) {
+  const uint32_t kind = Q8 ? (2u << 4) | (1u << 7) | (1u << 10) : 1u << 4;
+  return kind | (mn ? 3u << 15 : 0u) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+// MN-major operand in 64-byte swizzled atoms: blocks of 64 bytes along MN (a
+// block's 128 rows are 8 KB), 8-row K groups 512 bytes apart
+__device__ __forceinline__ uint64_t sw64_desc_mn(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)(8192 >> 4) << 16 | (uint64_t)(512 >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)4 << 61;
+}
+// byte offset of 16-byte piece c of row r of such an operand
+__device__ __forceinline__ int sw64(int r, int c) { return (c >> 2) * 8192 + r * 64 + (((c & 3) ^ ((r >> 1) & 3)) << 4); }
+
+__device__ __forceinline__ float redux_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// pairs of floats, one instruction for both
+struct F2 {
+  unsigned long long v;
+  __device__ __forceinline__ F2() {}
+  __device__ __forceinline__ F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ explicit F2(float a) : F2(a, a) {}
+  __device__ __forceinline__ float lo() const {
+    float a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+    return a;
+  }
+  __device__ __forceinline__ float hi() const {
+    float a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+    return b;
+  }
+};
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+// two integers in [-2^22, 2^22) as floats, without the conversion unit
+__device__ __forceinline__ F2 small_ints(uint32_t a, uint32_t b) {
+  return F2(__uint_as_float(a + 0x4B400000u), __uint_as_float(b + 0x4B400000u)) + F2(-12582912.0f);
+}
+template <int W>
+__device__ __forceinline__ void tt_ld(uint32_t taddr, uint32_t* r) {
+  if constexpr (W == 8) tc_ld8(taddr, r);
+  else tc_ld16(taddr, r);
+}
+// Columns c, c + 1 of W loaded from an accumulator: the three digits' sums put together, or head + remainder
+template <bool Q8, int W>
+__device__ __forceinline__ F2 joined(const uint32_t* v, int c) {
+  const uint32_t *v1 = v + W, *v2 = v + 2 * W;
+  if constexpr (Q8) {
+    const F2 k(256.0f);
+    return fma2(fma2(small_ints(v[c], v[c + 1]), k, small_ints(v1[c], v1[c + 1])), k, small_ints(v2[c], v2[c + 1]));
+  } else {
+    return F2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])) + F2(__uint_as_float(v1[c]), __uint_as_float(v1[c + 1]));
+  }
+}
+// A bounded wait.  Once any role of the CTA has given up, every wait returns at
+// once: the loops run on to their ends, so that named barriers stay matched.
+// Each try may suspend for 20 us: a spinning warp takes issue slots from the rest.
+constexpr uint32_t TT_POLLS = 1u << 17;
+__device__ __forceinline__ void tt_wait(uint64_t* bar, uint32_t phase, volatile int* abort) {
+  for (uint32_t i = 0; i < TT_POLLS; i++) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(phase), "r"(20000u)
+        : "memory");
+    if (ok) return;
+    if (*abort) return;
+  }
+  *abort = 1;
+}
+__device__ __forceinline__ void group_sync(int g) { asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory"); }
+__device__ __forceinline__ void groups_sync() { asm volatile("bar.sync 5, 512;" ::: "memory"); }
+__device__ __forceinline__ bool groups_any(bool pred) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.or.pred q, 5, 512, p;\n selp.u32 %0, 1, 0, q;\n}"
+      : "=r"(r)
+      : "r"((uint32_t)pred)
+      : "memory");
+  return r != 0;
+}
+
+__device__ __forceinline__ int tree_tiles(const TreeSeq& s) { return (s.len + s.n + TT_TILE - 1) / TT_TILE; }
+__device__ __forceinline__ int tree_chunks(const TreeSeq& s, int group, int ch) { return (s.n * group + ch - 1) / ch; }
+__device__ __forceinline__ unsigned long long tree_work(const TreeSeq& s, int n_kv, int group, int ch) {
+  return s.n ? (unsigned long long)tree_tiles(s) * tree_chunks(s, group, ch) * n_kv : 0ull;
+}
+
+// A CTA's walk over its share: segments of consecutive tiles of one unit.
+struct TreeWalk {
+  const TreeArgs* a;
+  TreeSeq s;
+  int b, kvh, chunk, tile, tiles, chunks, group, ch;
+  int left;  // tiles of the share still to go, this segment's included
+  int seg;   // tiles of this segment
+  __device__ __forceinline__ void start(const TreeArgs* args, int ch_, int seq, unsigned long long at, int n) {
+    a = args;
+    ch = ch_;
+    group = a->n_heads / a->c.n_kv;
+    b = seq;
+    left = n;
+    load();
+    tile = (int)(at % tiles);
+    const unsigned long long u = at / tiles;
+    chunk = (int)(u % chunks);
+    kvh = (int)(u / chunks);
+    seg = min(left, tiles - tile);
+  }
+  __device__ __forceinline__ void load() {
+    s = tree_seq(*a, b);
+    while (!s.n && b + 1 < a->n_seq) s = tree_seq(*a, ++b);
+    tiles = max(1, tree_tiles(s));
+    chunks = max(1, tree_chunks(s, group, ch));
+  }
+  __device__ __forceinline__ bool next() {  // false: the share is done
+    left -= seg;
+    if (left <= 0) return false;
+    tile = 0;
+    if (++chunk == chunks) {
+      chunk = 0;
+      if (++kvh == a->c.n_kv) {
+        kvh = 0;
+        b++;
+        load();
+      }
+    }
+    seg = min(left, tiles);
+    return true;
+  }
+};
+
+// What the softmax groups need of a segment; places count from its first tile.
+struct TreeSegment {
+  int row, len, total, off;  // cache row of place 0; places all nodes see; places; first query row
+  int kvh, tiles;
+  int first, rest;           // does the unit begin here; its tiles after this segment
+  int vh0, cols;             // the chunk's first column of the unit, and its columns
+  int more;                  // another segment follows
+};
+
+template <bool Q8, int NQ, int CG>
+__global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_constant__ TreeTcArgs ta) {
+  using S = TtShape<Q8, NQ, CG>;
+  constexpr int CH = S::CH, TG = S::TG, N = S::N, CS = S::CS;
+  const TreeArgs& a = ta.t;
+  extern __shared__ __align__(16) uint8_t smem_dyn[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~(uintptr_t)1023);
+  uint8_t* q_t = base + S::OFF_Q;
+  __shared__ __align__(8) uint64_t full[TT_MAX_SLOTS], empty[TT_MAX_SLOTS], s_full[4], s_free[4], p_full[4], o_full[4], q_ready, q_free, t_free, done_s, done_o;
+  __shared__ uint32_t tmem_s;
+  __shared__ int s_abort;
+  // a segment and its columns, in one of two sets: the nodes a column's node sees,
+  // its place in the sequence's q and out rows, its score factor; and the nodes
+  // some column sees
+  __shared__ TreeSegment seg_tab[2];
+  __shared__ unsigned long long col_mask[2][CH], any_mask[2];
+  __shared__ int col_off[2][CH];
+  __shared__ __align__(16) float col_mul[2][CH];
+  __shared__ __align__(16) float x_max[4][2][4][NQ], x_sum[4][4][NQ];
+  __shared__ __align__(16) float x_m[16][NQ], x_w[16][NQ], x_al[16][NQ], x_fold[16][2][NQ];  // per warp
+  __shared__ float2 x_fin[4][NQ];              // (max, sum) of a finished segment
+  __shared__ unsigned long long x_bad[4][2];   // drafted rows of V that are not finite
+  __shared__ unsigned long long w_sum[TT_THREADS / 32], s_total, s_at, s_all;
+  __shared__ int s_seq;
+  volatile int* abort = &s_abort;
+
+  const int tid = threadIdx.x, lane = tid & 31, wi = tid >> 5;
+  const int hd = a.c.hd, n_kv = a.c.n_kv, group = a.n_heads / n_kv;
+  const int slots = ta.slots, boxes = ta.boxes;
+  const uint32_t slot_bytes = (uint32_t)boxes * 16384u;
+
+  if (tid == 0) {
+    s_abort = 0;
+    for (int i = 0; i < slots; i++) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int g = 0; g < TG; g++) {
+      mbar_init(&s_full[g], 1);
+      mbar_init(&s_free[g], 128 * CG);
+      mbar_init(&p_full[g], 128 * CG);
+      mbar_init(&o_full[g], 1);
+    }
+    mbar_init(&q_ready, 32);
+    mbar_init(&q_free, 1);
+    mbar_init(&t_free, TT_SOFT);
+    mbar_init(&done_s, 1);
+    mbar_init(&done_o, 1);
+    fence_barrier_init();
+  }
+  pdl_wait();     // what comes next reads what earlier kernels wrote
+  pdl_trigger();  // the merge kernel may take its place; it waits for this grid
+  if (wi == TT_S_WARP) {  // after the wait: an earlier kernel may still have needed the TMEM
+    tc_alloc(&tmem_s, S::TMEM);
+    tc_relinquish();
+  }
+
+  // ---- this CTA's share of the tiles
+  {
+    const int n_seq = a.n_seq;
+    auto work = [&](int b) { return b < n_seq ? tree_work(tree_seq(a, b), n_kv, group, CH) : 0ull; };
+    const unsigned long long mine = work(tid);
+    unsigned long long sum = mine;
+    for (int b = tid + TT_THREADS; b < n_seq; b += TT_THREADS) sum += work(b);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) w_sum[wi] = sum;
+    __syncthreads();
+    unsigned long long total = 0;
+    for (int w = 0; w < TT_THREADS / 32; w++) total += w_sum[w];
+    // no more shares than tiles, so that every share between two others holds something
+    const unsigned long long shares = total < gridDim.x ? total : gridDim.x;
+    const unsigned long long t0 = blockIdx.x < shares ? total * blockIdx.x / shares : total;
+    const unsigned long long t1 = blockIdx.x < shares ? total * (blockIdx.x + 1) / shares : total;
+    if (tid == 0) {
+      s_total = t1 - t0;
+      s_all = total;
+      s_seq = 0;
+      s_at = 0;
+      ta.parts[blockIdx.x].n = 0;
+    }
+    const bool all = blockIdx.x == 0;  // CTA 0 looks for sequences that do not fit
+    unsigned long long before = 0;
+    for (int b0 = 0; b0 < n_seq && (all || (t1 > t0 && before <= t0)); b0 += TT_THREADS) {
+      const int b = b0 + tid;
+      const unsigned long long w = b0 ? work(b) : mine;
+      unsigned long long inc = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long x = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += x;
+      }
+      __syncthreads();
+      if (lane == 31) w_sum[wi] = inc;
+      __syncthreads();
+      unsigned long long pre = before, chunk = 0;
+      for (int x = 0; x < TT_THREADS / 32; x++) {
+        if (x < wi) pre += w_sum[x];
+        chunk += w_sum[x];
+      }
+      pre += inc - w;
+      if (w && pre <= t0 && t0 < pre + w) {
+        s_seq = b;
+        s_at = t0 - pre;
+      }
+      if (all && b < n_seq && tree_seq_bad(a, b, tree_seq(a, b))) atomicOr(a.err, ERR_RANGE);
+      before += chunk;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_s;
+  const int n_tiles = (int)s_total;
+  // Team k % TG does the CTA's tile k, as its item k / TG.
+  if (n_tiles == 0) {
+    // nothing: fall through to the end
+  } else if (wi == TT_TMA_WARP) {
+    // ------------------------------------------------ TMA: K and V of every tile, slot after slot
+    if (lane == 0) {
+      TreeWalk w;
+      w.start(&a, CH, s_seq, s_at, n_tiles);
+      int slot = 0, used = 0;
+      uint32_t phase = 1;  // a fresh barrier's previous phase counts as done
+      bool go = true;
+      do {
+        for (int t = w.tile; go && t < w.tile + w.seg; t++)
+          for (int kv = 0; kv < 2; kv++) {
+            tt_wait(&empty[slot], phase, abort);
+            if (*abort) {
+              go = false;
+              break;
+            }
+            mbar_arrive_expect_tx(&full[slot], slot_bytes);
+            for (int x = 0; x < boxes; x++)
+              tma_load_3d(base + slot * slot_bytes + x * 16384, kv ? &ta.tm_v : &ta.tm_k, x * 64, w.kvh,
+                          w.s.start + t * TT_TILE, &full[slot]);
+            used++;
+            if (++slot == slots) {
+              slot = 0;
+              phase ^= 1;
+            }
+          }
+      } while (go && w.next());
+      // wind down: every copy issued has landed before the CTA may exit
+      for (int i = max(0, used - slots); i < used; i++)
+        if (!mbar_wait(&full[i % slots], (uint32_t)(i / slots) & 1, *abort ? 1u << 16 : kMbarPolls)) *abort = 1;
+    }
+    __syncwarp();
+  } else if (wi == TT_S_WARP || wi == TT_O_WARP) {
+    // ------------------------------------------------ MMA: scores (K slots), outputs (V slots)
+    if (lane == 0) {
+      TreeWalk w;
+      w.start(&a, CH, s_seq, s_at, n_tiles);
+      const bool scores = wi == TT_S_WARP;
+      const int ks_n = Q8 ? (hd + 31) / 32 : (hd + 15) / 16;
+      constexpr uint32_t IDESC_S = tt_idesc<Q8>(N, false), IDESC_O = tt_idesc<Q8>(N, true);
+      int slot = scores ? 0 : 1, seg_left = w.seg;
+      uint32_t phase = 0, segs = 0;
+      bool fresh = true;  // a segment begins: its columns first
+      for (int k = 0; k < n_tiles && !*abort; k++) {
+        const int g = k % TG;
+        const uint32_t n = (uint32_t)(k / TG);
+        if (scores) {
+          if (fresh) tt_wait(&q_ready, segs & 1, abort);
+          if (n) tt_wait(&s_free[g], (n - 1) & 1, abort);
+          tt_wait(&full[slot], phase, abort);
+          if (*abort) break;
+          tc_fence_after();
+          const uint64_t kd = sw128_desc(smem_u32(base + slot * slot_bytes));
+          const uint64_t qd = sw128_desc(smem_u32(q_t));
+          // unrolled: a product whose descriptors and flags the compiler does not
+          // know takes 125 cycles to issue, not 40
+#pragma unroll
+          for (int ks = 0; ks < (Q8 ? 4 : 8); ks++) {
+            if (ks >= ks_n) break;
+            if constexpr (Q8)
+              tc_mma_i8_acc(tmem + g * CS, kd + ks * 2, qd + ks * 2, IDESC_S, ks > 0);
+            else
+              tc_mma_f16(tmem + g * CS, kd + (uint64_t)((ks >> 2) * 1024 + (ks & 3) * 2),
+                         qd + (uint64_t)((ks >> 2) * (N * 8) + (ks & 3) * 2), IDESC_S, ks > 0);
+          }
+          tc_commit(&s_full[g]);
+          fresh = --seg_left == 0;
+          if (fresh) {
+            tc_commit(&q_free);
+            segs++;
+            if (k + 1 < n_tiles) w.next();
+            seg_left = w.seg;
+          }
+        } else {
+          tt_wait(&p_full[g], n & 1, abort);
+          tt_wait(&full[slot], phase, abort);
+          if (*abort) break;
+          tc_fence_after();
+          // one 128-byte-wide block of M per box; a lone f16 box stands for both
+          // halves (the upper half of O is not read)
+          const uint64_t vd = sw128_desc_mn(smem_u32(base + slot * slot_bytes), boxes == 2 ? 16384u : 0u, 1024u);
+          const uint64_t pd = sw64_desc_mn(smem_u32(base + S::OFF_P + g * S::PSZ));
+          constexpr int STEPS = Q8 ? 4 : 8;  // 32 or 16 positions each
+#pragma unroll
+          for (int ks = 0; ks < STEPS; ks++) {
+            if constexpr (Q8)
+              tc_mma_i8_acc(tmem + (TG + g) * CS, vd + ks * 256, pd + ks * 128, IDESC_O, ks > 0);
+            else
+              tc_mma_f16(tmem + (TG + g) * CS, vd + ks * 128, pd + ks * 64, IDESC_O, ks > 0);
+          }
+          tc_commit(&o_full[g]);
+        }
+        tc_commit(&empty[slot]);
+        slot += 2;  // K and V alternate
+        if (slot >= slots) {
+          slot -= slots;
+          phase ^= 1;
+        }
+      }
+      // wind down: every MMA issued has completed before TMEM is freed
+      uint64_t* last = scores ? &done_s : &done_o;
+      tc_commit(last);
+      if (!mbar_wait(last, 0, *abort ? 1u << 16 : kMbarPolls)) *abort = 1;
+    }
+    __syncwarp();
+  } else if (wi == TT_Q_WARP) {
+    // ------------------------------------------------ the next segment's columns: q operand, masks, places
+    const float scale2 = LOG2E / sqrtf((float)hd);
+    TreeWalk w;
+    w.start(&a, CH, s_seq, s_at, n_tiles);
+    int seg = 0;
+    bool more;
+    do {
+      const int set = seg & 1, cols = min(CH, w.s.n * group - w.chunk * CH);
+      const float* q_seq = a.q + (size_t)w.s.off * a.n_heads * hd;
+      if (seg >= 2) tt_wait(&t_free, (uint32_t)seg & 1, abort);  // the set's readers, two segments ago
+      if (*abort) break;
+      TreeSegment sg{w.s.start + w.tile * TT_TILE, w.s.len - w.tile * TT_TILE, w.s.len + w.s.n - w.tile * TT_TILE, w.s.off,
+                     w.kvh, w.seg, w.tile == 0, w.tiles - w.tile - w.seg, w.chunk * CH, cols, 0};
+      if (lane == 0) any_mask[set] = 0ull;
+      bool q_mine = seg == 0;
+      for (int cb = 0; cb < CH; cb += 4) {
+        float x[4][4];
+        unsigned long long mask[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {  // four columns' loads at once
+          const int vh = w.chunk * CH + cb + u, node = vh / group, head = w.kvh * group + vh % group;
+          const bool in = cb + u < cols;
+          const int off = (node * a.n_heads + head) * hd;
+          mask[u] = in ? tree_mask(a, w.s, node) : 0ull;
+          if (lane == 0) col_off[set][cb + u] = off;
+#pragma unroll
+          for (int e = 0; e < 4; e++) x[u][e] = in && lane * 4 + e < hd ? q_seq[off + lane * 4 + e] : 0.0f;
+        }
+        if (!q_mine) {  // the last segment's products have read the operand
+          tt_wait(&q_free, (uint32_t)(seg - 1) & 1, abort);
+          q_mine = true;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          const int c = cb + u;
+          float amax = 0.0f;
+          bool nan = false;
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            nan |= x[u][e] != x[u][e];
+            amax = fmaxf(amax, fabsf(x[u][e]));
+          }
+          amax = redux_max(amax);
+          nan = __any_sync(0xffffffffu, nan);
+          float mul;
+          if constexpr (Q8) {
+            const float up = amax < 1e-25f ? 0x1p96f : 1.0f;  // keeps the quotient finite
+            const float inv = amax > 0.0f ? TT_DIGITS / (amax * up) : 0.0f;
+            mul = (amax / TT_DIGITS) * scale2;
+            uint32_t dig[3] = {0u, 0u, 0u};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const int v = __float2int_rn(fminf(fmaxf(x[u][e] * up * inv, -TT_DIGITS), TT_DIGITS));
+              const uint32_t b = (uint32_t)(v + 0x808080) ^ 0x808080u;  // balanced digits, a byte each
+#pragma unroll
+              for (int z = 0; z < 3; z++) dig[z] |= (b >> (16 - 8 * z) & 255u) << (8 * e);
+            }
+#pragma unroll
+            for (int z = 0; z < 3; z++) {
+              const int row = z * CH + c;
+              *reinterpret_cast<uint32_t*>(q_t + row * 128 + (((lane >> 2) ^ (row & 7)) << 4) + (lane & 3) * 4) = dig[z];
+            }
+          } else {
+            // a power of two that brings the largest value to [2^13, 2^14)
+            const int e2 = amax > 0.0f && amax < INFINITY ? min(120, 13 - ilogbf(amax)) : 0;
+            const float up = __int_as_float((e2 + 127) << 23);
+            mul = scale2 / up;
+            alignas(8) __half hh[4], hl[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const float v = x[u][e] * up;
+              hh[e] = __float2half_rn(v);
+              hl[e] = __float2half_rn(v - __half2float(hh[e]));
+            }
+#pragma unroll
+            for (int z = 0; z < 2; z++) {
+              const int row = z * CH + c, k = lane * 4;
+              *reinterpret_cast<uint2*>(q_t + (k >> 6) * (N * 128) + row * 128 + ((((k & 63) >> 3) ^ (row & 7)) << 4) + (k & 7) * 2) =
+                  *reinterpret_cast<const uint2*>(z ? hl : hh);
+            }
+          }
+          if (lane == 0) {
+            col_mul[set][c] = nan ? __int_as_float(0x7fffffff) : mul;
+            col_mask[set][c] = mask[u];
+            any_mask[set] |= mask[u];
+          }
+        }
+      }
+      if constexpr (Q8 && NQ == 8) {  // the operand's last eight rows
+        for (int i = lane; i < 64; i += 32) *reinterpret_cast<uint4*>(q_t + 24 * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+      }
+      more = w.next();
+      sg.more = more;
+      if (lane == 0) seg_tab[set] = sg;
+      fence_async_smem();
+      mbar_arrive(&q_ready);
+      seg++;
+    } while (more && !*abort);
+  } else {
+    // ------------------------------------------------ softmax groups
+    const int g = wi >> 2, wq = wi & 3, r = tid & 127, tg = g / CG, cg = g % CG;
+    const uint32_t lanes = (uint32_t)(wq * 32) << 16;
+    const int c0 = cg * NQ;  // of the team's columns
+    const uint32_t s_at = tmem + lanes + (uint32_t)(tg * CS + c0), o_at = tmem + lanes + (uint32_t)((TG + tg) * CS + c0);
+    uint8_t* p_t = base + S::OFF_P + tg * S::PSZ;
+    const bool has_dim = wq * 32 < hd;  // this warp's lanes of O are dims
+    int item = 0;  // of this group, over all segments
+    int k0 = 0;    // tiles of the CTA before this segment
+    int seg_no = 0, more;
+    do {
+      const int set = seg_no & 1;
+      tt_wait(&q_ready, (uint32_t)seg_no & 1, abort);  // the segment and its columns' tables
+      // one decision for all, so that the named barriers stay matched; from here
+      // on the last segment's p operands are free
+      if (groups_any(*abort != 0)) break;
+      const TreeSegment& sg = seg_tab[set];
+      const int len = sg.len, total = sg.total, tiles = sg.tiles;
+      const int first = (tg - k0) & (TG - 1);
+      const float *ks_at = nullptr, *vs_at = nullptr;
+      float ks_next = 0.0f, vs_next = 0.0f;
+      auto scales = [&](int t) {  // of tile t's place r, and on to the group's next tile
+        const bool in = t * TT_TILE + r < total;
+        ks_next = in ? __ldg(ks_at) : 0.0f;
+        vs_next = in ? __ldg(vs_at) : 0.0f;
+        ks_at += (size_t)(TG * TT_TILE) * a.c.scale_row;
+        vs_at += (size_t)(TG * TT_TILE) * a.c.scale_row;
+      };
+      if (Q8 && first < tiles) {
+        const size_t at = ((size_t)sg.row + first * TT_TILE + r) * a.c.scale_row + (size_t)sg.kvh * a.c.scale_head;
+        ks_at = a.c.k_scale + at;
+        vs_at = a.c.v_scale + at;
+        scales(first);
+      }
+      F2 l[NQ / 2], o[NQ / 2];
+      float R = -INFINITY;  // lane c holds the running maximum of column c
+#pragma unroll
+      for (int c = 0; c < NQ / 2; c++) l[c] = o[c] = F2(0.0f);
+
+      // O of the group's previous item into the registers
+      auto fold = [&](int par) {
+        tt_wait(&o_full[tg], (uint32_t)(item - 1) & 1, abort);
+        tc_fence_after();
+        if (has_dim) {
+#pragma unroll
+          for (int cb = 0; cb < NQ; cb += 8) {
+            uint32_t v[24];
+            tt_ld<8>(o_at + cb, v);
+            tt_ld<8>(o_at + CH + cb, v + 8);
+            if constexpr (Q8) tt_ld<8>(o_at + 2 * CH + cb, v + 16);
+            tc_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 8; c += 4) {
+              const float4 f = *reinterpret_cast<const float4*>(&x_fold[wi][par][cb + c]);
+              F2& o0 = o[(cb + c) / 2];
+              F2& o1 = o[(cb + c) / 2 + 1];
+              o0 = fma2(joined<Q8, 8>(v, c), F2(f.x, f.y), o0);
+              o1 = fma2(joined<Q8, 8>(v, c + 2), F2(f.z, f.w), o1);
+            }
+          }
+        }
+        tc_fence_before();
+        if constexpr (!Q8) {  // drafted rows of V that are not finite: nodes that see them get NaN
+          unsigned long long bad = x_bad[g][par];
+          while (bad) {
+            const int j = __ffsll((long long)bad) - 1;
+            bad &= bad - 1;
+            float v = 0.0f;
+            if (r < hd)
+              v = __half2float(static_cast<const __half*>(a.c.v)[(size_t)(sg.row + len + j) * a.c.row_stride +
+                                                                (size_t)sg.kvh * a.c.head_stride + r]);
+            if (!(fabsf(v) < INFINITY)) {
+              const float nan = __int_as_float(0x7fffffff);
+#pragma unroll
+              for (int c = 0; c < NQ; c += 2)
+                o[c / 2] = F2(col_mask[set][c0 + c] >> j & 1 ? nan : o[c / 2].lo(),
+                              col_mask[set][c0 + c + 1] >> j & 1 ? nan : o[c / 2].hi());
+            }
+          }
+        }
+      };
+
+      int done = 0;  // items of this segment
+      for (int t = first; t < tiles; t += TG, item++, done++) {
+        const int par = item & 1, pos = t * TT_TILE + r, j = pos - len;
+        const bool edge = (t + 1) * TT_TILE > len;  // drafted places or none at all among the tile's
+        const bool there = pos < total;
+        // an f16 edge tile: which 8-value pieces of this drafted V row are not finite
+        uint32_t odd = 0;
+        if constexpr (!Q8) {
+          if (edge) {
+            if (r == 0) x_bad[g][par] = 0ull;
+            if (there && j >= 0 && (any_mask[set] >> j & 1)) {
+              const uint4* v = reinterpret_cast<const uint4*>(static_cast<const __half*>(a.c.v) +
+                                                              (size_t)(sg.row + pos) * a.c.row_stride +
+                                                              (size_t)sg.kvh * a.c.head_stride);
+              for (int c = 0; c < hd / 8; c++) {
+                const uint4 x = v[c];
+                const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+                bool bad = false;
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                  bad |= (xs[e] & 0x7c00u) == 0x7c00u || (xs[e] & 0x7c000000u) == 0x7c000000u;
+                odd |= (uint32_t)bad << c;
+              }
+            }
+          }
+        }
+        // this place's scales: K's, and V's as 2^ve * vm
+        float ks = ks_next, vm = 0.0f;
+        int ve = 0;
+        if constexpr (Q8) {
+          const float vs = vs_next;
+          if (t + TG < tiles) scales(t + TG);
+          const uint32_t b = __float_as_uint(vs);
+          if (b >= 0x7f800000u) {  // negative, infinite or NaN: whoever sees the place gets NaN
+            ks = __int_as_float(0x7fffffff);
+          } else if (b < 0x00800000u) {
+            ve = -126;
+            vm = vs * 0x1p126f;
+          } else {
+            ve = (int)(b >> 23) - 127;
+            vm = __uint_as_float((b & 0x007fffffu) | 0x3f800000u);
+          }
+        }
+        // ---- scores (with V's exponent), in powers of two
+        tt_wait(&s_full[tg], (uint32_t)item & 1, abort);
+        tc_fence_after();
+        constexpr int W = NQ;  // columns of one load: each wait for TMEM costs its whole latency
+        F2 s[NQ / 2];
+        const F2 ks2(ks), ve2((float)ve);
+#pragma unroll
+        for (int cb = 0; cb < NQ; cb += W) {
+          uint32_t v[3 * W];
+          tt_ld<W>(s_at + cb, v);
+          tt_ld<W>(s_at + CH + cb, v + W);
+          if constexpr (Q8) tt_ld<W>(s_at + 2 * CH + cb, v + 2 * W);
+          tc_wait_ld();
+#pragma unroll
+          for (int c = 0; c < W; c += 4) {
+            const float4 m = *reinterpret_cast<const float4*>(&col_mul[set][c0 + cb + c]);
+            F2& s0 = s[(cb + c) / 2];
+            F2& s1 = s[(cb + c) / 2 + 1];
+            if constexpr (Q8) {
+              s0 = fma2(joined<Q8, W>(v, c), F2(m.x, m.y) * ks2, ve2);
+              s1 = fma2(joined<Q8, W>(v, c + 2), F2(m.z, m.w) * ks2, ve2);
+            } else {
+              s0 = joined<Q8, W>(v, c) * F2(m.x, m.y);
+              s1 = joined<Q8, W>(v, c + 2) * F2(m.z, m.w);
+            }
+          }
+        }
+        tc_fence_before();
+        mbar_arrive(&s_free[tg]);
+        if (edge) {
+#pragma unroll
+          for (int c = 0; c < NQ; c += 2) {
+            const bool s0 = j < 0 || (there && (col_mask[set][c0 + c] >> j & 1));
+            const bool s1 = j < 0 || (there && (col_mask[set][c0 + c + 1] >> j & 1));
+            s[c / 2] = F2(s0 ? s[c / 2].lo() : -INFINITY, s1 ? s[c / 2].hi() : -INFINITY);
+          }
+        }
+        // ---- the tile's maximum of every column
+#pragma unroll
+        for (int c = 0; c < NQ; c += 4) {
+          float4 m;
+          m.x = redux_max(s[c / 2].lo());
+          m.y = redux_max(s[c / 2].hi());
+          m.z = redux_max(s[c / 2 + 1].lo());
+          m.w = redux_max(s[c / 2 + 1].hi());
+          if (lane == 0) *reinterpret_cast<float4*>(&x_max[g][par][wq][c]) = m;
+        }
+        group_sync(g);
+        float al = 1.0f;
+        if (lane < NQ) {
+          const float m = fmaxf(fmaxf(x_max[g][par][0][lane], x_max[g][par][1][lane]),
+                                fmaxf(x_max[g][par][2][lane], x_max[g][par][3][lane]));
+          const float top = fmaxf(R, m);
+          const float wt = m == -INFINITY ? 0.0f : ex2(m - top);
+          if (R != -INFINITY) al = ex2(R - top);
+          R = top;
+          x_m[wi][lane] = m == -INFINITY ? 0.0f : -m;
+          x_w[wi][lane] = wt;
+          x_al[wi][lane] = al;
+          x_fold[wi][par][lane] = wt * (Q8 ? 2.0f / TT_DIGITS : 0x1p-15f);
+        }
+        const bool moved = __any_sync(0xffffffffu, al != 1.0f);
+        if (done) fold(par ^ 1);
+        __syncwarp();
+        if (moved) {
+#pragma unroll
+          for (int c = 0; c < NQ; c += 2) {
+            const F2 f(x_al[wi][c], x_al[wi][c + 1]);
+            l[c / 2] = l[c / 2] * f;
+            o[c / 2] = o[c / 2] * f;
+          }
+        }
+        // ---- probabilities, in the operand's form, a row per position
+        if constexpr (Q8) {
+          const bool tiny = ve < -60;  // such a place's weight may be lost beside p * 2^ve: it is summed by itself
+          if (__any_sync(0xffffffffu, tiny)) {
+#pragma unroll
+            for (int c = 0; c < NQ; c += 2) {
+              const float p0 = tiny ? ex2((s[c / 2].lo() + x_m[wi][c]) - (float)ve) : 0.0f;
+              const float p1 = tiny ? ex2((s[c / 2].hi() + x_m[wi][c + 1]) - (float)ve) : 0.0f;
+              l[c / 2] = fma2(F2(p0, p1), F2(x_w[wi][c], x_w[wi][c + 1]), l[c / 2]);
+            }
+          }
+          const F2 cm(vm * (0.5f * TT_DIGITS)), iv(tiny ? 0.0f : __uint_as_float((uint32_t)(127 - ve) << 23)), bias(TT_BIAS);
+          uint32_t dg[3][NQ / 4];
+#pragma unroll
+          for (int c = 0; c < NQ; c += 4) {
+            const float4 m = *reinterpret_cast<const float4*>(&x_m[wi][c]);
+            const float4 wt = *reinterpret_cast<const float4*>(&x_w[wi][c]);
+            const F2 d0 = s[c / 2] + F2(m.x, m.y), d1 = s[c / 2 + 1] + F2(m.z, m.w);
+            const F2 p0(ex2(d0.lo()), ex2(d0.hi())), p1(ex2(d1.lo()), ex2(d1.hi()));
+            l[c / 2] = fma2(p0 * iv, F2(wt.x, wt.y), l[c / 2]);
+            l[c / 2 + 1] = fma2(p1 * iv, F2(wt.z, wt.w), l[c / 2 + 1]);
+            const F2 f0 = fma2(p0, cm, bias), f1 = fma2(p1, cm, bias);
+            const uint32_t f[4] = {__float_as_uint(f0.lo()), __float_as_uint(f0.hi()), __float_as_uint(f1.lo()),
+                                   __float_as_uint(f1.hi())};
+            const uint32_t a01 = __byte_perm(f[0], f[1], 0x5140), a23 = __byte_perm(f[2], f[3], 0x5140);
+            dg[2][c / 4] = __byte_perm(a01, a23, 0x5410) ^ 0x80808080u;
+            dg[1][c / 4] = __byte_perm(a01, a23, 0x7632) ^ 0x80808080u;
+            dg[0][c / 4] = __byte_perm(__byte_perm(f[0], f[1], 0x0062), __byte_perm(f[2], f[3], 0x0062), 0x5410);
+          }
+          if constexpr (NQ == 16) {
+#pragma unroll
+            for (int z = 0; z < 3; z++)
+              *reinterpret_cast<uint4*>(p_t + sw64(r, z * CG + cg)) = make_uint4(dg[z][0], dg[z][1], dg[z][2], dg[z][3]);
+          } else {
+            *reinterpret_cast<uint4*>(p_t + sw64(r, 0)) = make_uint4(dg[0][0], dg[0][1], dg[1][0], dg[1][1]);
+            *reinterpret_cast<uint4*>(p_t + sw64(r, 1)) = make_uint4(dg[2][0], dg[2][1], 0u, 0u);
+          }
+        } else {
+#pragma unroll
+          for (int cb = 0; cb < NQ; cb += 8) {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const int c = cb + e * 2;
+              const F2 d = s[c / 2] + F2(x_m[wi][c], x_m[wi][c + 1]);
+              const F2 p(ex2(d.lo()), ex2(d.hi()));
+              l[c / 2] = fma2(p, F2(x_w[wi][c], x_w[wi][c + 1]), l[c / 2]);
+              const F2 x = p * F2(32768.0f);  // far from f16's smallest values
+              const F2 h(__uint_as_float(__float_as_uint(x.lo()) & 0xffffe000u), __uint_as_float(__float_as_uint(x.hi()) & 0xffffe000u));
+              const F2 rest = fma2(h, F2(-1.0f), x);
+              const __half2 hh = __floats2half2_rn(h.lo(), h.hi()), dd = __floats2half2_rn(rest.lo(), rest.hi());
+              hi[e] = *reinterpret_cast<const uint32_t*>(&hh);
+              lo[e] = *reinterpret_cast<const uint32_t*>(&dd);
+            }
+            *reinterpret_cast<uint4*>(p_t + sw64(r, (c0 + cb) / 8)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4*>(p_t + sw64(r, (CH + c0 + cb) / 8)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          }
+          // V of places nobody sees, and values that are not finite in drafted rows, become zeros
+          if (edge) {
+            const int v_no = 2 * (k0 + t) + 1;  // K and V alternate over the CTA's tiles
+            const bool row_gone = j >= 0 && !(there && (any_mask[set] >> j & 1));
+            if (row_gone || odd) {
+              tt_wait(&full[v_no % slots], (uint32_t)(v_no / slots) & 1, abort);
+              uint8_t* vt = base + (v_no % slots) * slot_bytes + r * 128;
+              for (int c = 0; c < 8 * boxes; c++)
+                if (row_gone || (odd >> c & 1)) {
+                  uint4* at = reinterpret_cast<uint4*>(vt + (c >> 3) * 16384 + (((c & 7) ^ (r & 7)) << 4));
+                  if (row_gone) {
+                    *at = make_uint4(0u, 0u, 0u, 0u);
+                  } else {
+                    uint4 x = *at;
+                    uint32_t* xs = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                      if ((xs[e] & 0x7c00u) == 0x7c00u) xs[e] &= 0xffff0000u;
+                      if ((xs[e] & 0x7c000000u) == 0x7c000000u) xs[e] &= 0xffffu;
+                    }
+                    *at = x;
+                  }
+                }
+              if (odd) atomicOr(&x_bad[g][par], 1ull << j);
+            }
+          } else if (r == 0) {
+            x_bad[g][par] = 0ull;
+          }
+        }
+        fence_async_smem();
+        mbar_arrive(&p_full[tg]);
+        if constexpr (!Q8) group_sync(g);  // x_bad is whole before the fold reads it
+      }
+      if (done) fold((item - 1) & 1);
+
+      // ---- the segment's (max, sum, o): the groups of a column range meet through their idle p operands
+#pragma unroll
+      for (int c = 0; c < NQ; c += 4) {
+        const float4 x = make_float4(warp_sum(l[c / 2].lo()), warp_sum(l[c / 2].hi()), warp_sum(l[c / 2 + 1].lo()),
+                                     warp_sum(l[c / 2 + 1].hi()));
+        if (lane == 0) *reinterpret_cast<float4*>(&x_sum[g][wq][c]) = x;
+      }
+      if constexpr (TG > 1) {
+        float* po = reinterpret_cast<float*>(p_t) + cg * NQ * 128;
+#pragma unroll
+        for (int c = 0; c < NQ; c++) po[c * 128 + r] = c & 1 ? o[c / 2].hi() : o[c / 2].lo();
+      }
+      group_sync(g);
+      if (wq == 0 && lane < NQ)
+        x_fin[g][lane] = make_float2(R, (x_sum[g][0][lane] + x_sum[g][1][lane]) + (x_sum[g][2][lane] + x_sum[g][3][lane]));
+      groups_sync();
+      {
+        const bool whole = sg.first && !sg.rest;
+        const size_t slot = 2 * (size_t)blockIdx.x + (sg.first ? 1 : 0);
+        const int cols = sg.cols;
+        float* out_seq = a.out + (size_t)sg.off * a.n_heads * hd;
+        auto put = [&](int c, float m, float sum, float x) {  // column c: final, or a partial
+          if (whole) {
+            if (r < hd) out_seq[col_off[set][c0 + c] + r] = sum == 0.0f ? 0.0f : x / sum;
+          } else {
+            if (r == 0) ta.part_ml[slot * CH + c0 + c] = make_float2(m, sum);
+            if (r < hd) ta.part_o[(slot * CH + c0 + c) * hd + r] = x;
+          }
+        };
+        if constexpr (TG == 1) {
+#pragma unroll
+          for (int c = 0; c < NQ; c++)
+            if (c0 + c < cols) put(c, x_fin[g][c].x, x_fin[g][c].y, c & 1 ? o[c / 2].hi() : o[c / 2].lo());
+        } else {
+          for (int c = tg; c < NQ && c0 + c < cols; c += TG) {  // the teams share the columns
+            float m = -INFINITY, sum = 0.0f, x = 0.0f;
+#pragma unroll
+            for (int q = 0; q < TG; q++) m = fmaxf(m, x_fin[q * CG + cg][c].x);
+#pragma unroll
+            for (int q = 0; q < TG; q++) {
+              const float2 f = x_fin[q * CG + cg][c];
+              const float wt = f.x == -INFINITY ? 0.0f : ex2(f.x - m);
+              sum = fmaf(f.y, wt, sum);
+              x = fmaf(reinterpret_cast<const float*>(base + S::OFF_P + q * S::PSZ)[(c0 + c) * 128 + r], wt, x);
+            }
+            put(c, m, sum, x);
+          }
+        }
+        if (tid == 0 && sg.first && !whole) {  // the unit goes on in the next CTAs
+          const unsigned long long shares = s_all < gridDim.x ? s_all : gridDim.x;
+          const unsigned long long t1 = s_all * (blockIdx.x + 1) / shares;  // the end of this share
+          const unsigned long long u1 = t1 + (unsigned long long)sg.rest;
+          TreePart* pt = ta.parts + blockIdx.x;
+          pt->cols = cols;
+          pt->vh0 = sg.vh0;
+          pt->kvh = sg.kvh;
+          pt->off = sg.off;
+          pt->n = (int)((u1 * shares - 1) / s_all) - (int)blockIdx.x + 1;
+        }
+      }
+      more = sg.more;
+      mbar_arrive(&t_free);
+      k0 += tiles;
+      seg_no++;
+    } while (more);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (tid == 0 && *abort) atomicOr(a.err, ERR_TIMEOUT);
+  if (wi == TT_S_WARP) tc_dealloc(tmem, S::TMEM);
+}
+
+// The units that several CTAs shared, each found at the CTA it began in: one
+// warp per column sums the partials in the order of the tiles.
+__global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__ TreeTcArgs ta, int ch) {
+  const TreeArgs& a = ta.t;
+  const int group = a.n_heads / a.c.n_kv, hd = a.c.hd, lane = threadIdx.x & 31;
+  const int i0 = blockIdx.x, c = blockIdx.y * 4 + (threadIdx.x >> 5);
+  pdl_wait();
+  pdl_trigger();
+  const TreePart u = ta.parts[i0];
+  if (c >= ch || !u.n || c >= u.cols) return;
+  auto slot = [&](int i) { return (2 * (size_t)(i0 + i) + (i == 0 ? 1 : 0)) * ch + c; };
+  float m = -INFINITY;
+  for (int i = lane; i < u.n; i += 32) m = fmaxf(m, __ldcg(&ta.part_ml[slot(i)]).x);
+  m = warp_max(m);
+  float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int ib = 0; ib < u.n; ib += 32) {
+    float wt = 0.0f;
+    if (ib + lane < u.n) {
+      const float2 f = __ldcg(&ta.part_ml[slot(ib + lane)]);
+      wt = f.x == -INFINITY ? 0.0f : ex2(f.x - m);
+      l = fmaf(f.y, wt, l);
+    }
+#pragma unroll 8
+    for (int i = 0; i < min(32, u.n - ib); i++) {
+      const float f = __shfl_sync(0xffffffffu, wt, i);
+      const float* po = ta.part_o + slot(ib + i) * hd;
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (e * 32 + lane < hd) o[e] = fmaf(__ldcg(po + e * 32 + lane), f, o[e]);
+    }
+  }
+  l = warp_sum(l);
+  const int vh = u.vh0 + c, node = vh / group, head = u.kvh * group + vh % group;
+  float* out = a.out + ((size_t)(u.off + node) * a.n_heads + head) * hd;
+#pragma unroll
+  for (int e = 0; e < 4; e++)
+    if (e * 32 + lane < hd) out[e * 32 + lane] = l == 0.0f ? 0.0f : o[e] / l;
+}
+
+static size_t al256(size_t x) { return (x + 255) & ~(size_t)255; }
+static int tt_columns(int max_nodes, int group) {
+  const int vh = max_nodes * group;
+  return vh <= 8 ? 8 : vh <= 16 ? 16 : vh <= 32 ? 32 : 64;
+}
+
+size_t tree_workspace_bytes(int max_nodes, int n_heads, int n_kv, int hd, int sm_count) {
+  const size_t cols = (size_t)2 * sm_count * tt_columns(max_nodes, n_heads / n_kv);
+  return al256(sm_count * sizeof(TreePart)) + al256(cols * 8) + al256(cols * hd * 4);
+}
+
+template <typename F>
+static cudaError_t tt_launch(F fn, dim3 grid, int threads, size_t smem, cudaStream_t st, void** args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelExC(&cfg, (const void*)fn, args);
+}
+
+template <bool Q8, int NQ, int CG>
+static cudaError_t tt_go(TreeTcArgs& ta, cudaStream_t st) {
+  using S = TtShape<Q8, NQ, CG>;
+  auto k = tree_tc_kernel<Q8, NQ, CG>;
+  cudaError_t e = cudaFuncSetAttribute((const void*)k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::BYTES);
+  if (e != cudaSuccess) return e;
+  ta.slots = S::RING / (ta.boxes * 16384);
+  if (ta.slots > TT_MAX_SLOTS) ta.slots = TT_MAX_SLOTS;
+  void* args[] = {&ta};
+  e = tt_launch(k, dim3(ta.t.sm_count), TT_THREADS, S::BYTES, st, args);
+  if (e != cudaSuccess) return e;
+  int ch = S::CH;
+  void* margs[] = {&ta, &ch};
+  return tt_launch(tree_merge_kernel, dim3(ta.t.sm_count, S::CH / 4), 128, 0, st, margs);
+}
 
 cudaError_t launch_attn_tree(const TreeArgs& a, cudaStream_t st) {
-  const dim3 grid((unsigned)a.n_seq, (unsigned)a.n_heads, (unsigned)a.max_nodes);
-  if (a.c.q8) tree_simple_kernel<true><<<grid, TR_THREADS, 0, st>>>(a);
-  else tree_simple_kernel<false><<<grid, TR_THREADS, 0, st>>>(a);
-  return cudaGetLastError();
+  TreeTcArgs ta;
+  const KvRowsDev& c = a.c;
+  const int box = c.q8 ? 128 : 64, group = a.n_heads / c.n_kv;
+  const bool maps = c.hd <= 128 &&
+                    encode_rows_map(&ta.tm_k, c.k, c.q8, c.positions, c.n_kv, c.hd, c.row_stride, c.head_stride, box) &&
+                    encode_rows_map(&ta.tm_v, c.v, c.q8, c.positions, c.n_kv, c.hd, c.row_stride, c.head_stride, box);
+  if (!maps) {
+    const dim3 grid((unsigned)a.n_seq, (unsigned)a.n_heads, (unsigned)a.max_nodes);
+    if (c.q8) tree_simple_kernel<true><<<grid, TR_THREADS, 0, st>>>(a);
+    else tree_simple_kernel<false><<<grid, TR_THREADS, 0, st>>>(a);
+    return cudaGetLastError();
+  }
+  ta.t = a;
+  ta.boxes = !c.q8 && c.hd > 64 ? 2 : 1;
+  const int cols = tt_columns(a.max_nodes, group);
+  const size_t n = (size_t)2 * a.sm_count * cols;
+  uint8_t* w = static_cast<uint8_t*>(a.work);
+  ta.parts = reinterpret_cast<TreePart*>(w);
+  w += al256(a.sm_count * sizeof(TreePart));
+  ta.part_ml = reinterpret_cast<float2*>(w);
+  ta.part_o = reinterpret_cast<float*>(w + al256(n * 8));
+  switch (cols) {
+    case 8: return c.q8 ? tt_go<true, 8, 1>(ta, st) : tt_go<false, 8, 1>(ta, st);
+    case 16: return c.q8 ? tt_go<true, 16, 1>(ta, st) : tt_go<false, 16, 1>(ta, st);
+    case 32: return c.q8 ? tt_go<true, 16, 2>(ta, st) : tt_go<false, 16, 2>(ta, st);
+    default: return c.q8 ? tt_go<true, 16, 4>(ta, st) : tt_go<false, 16, 4>(ta, st);
+  }
 }
 
 }  // namespace prana

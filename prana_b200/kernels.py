@@ -470,11 +470,11 @@ def attention_tree(q: torch.Tensor, cache: KvRows, starts: torch.Tensor, lens: t
     elif out.dtype != torch.float32 or out.device != device or not out.is_contiguous() or out.numel() != n_nodes * width:
         raise ValueError("out must be a contiguous float32 [n_nodes, n_heads * head_dim] on the cache's device")
     ctx = context(device.index)
-    key = (device.index, n_seq, max_nodes, n_heads, view.n_kv_heads, view.head_dim)
+    key = (device.index, max_nodes, n_heads, view.n_kv_heads, view.head_dim)
     size = _tree_work.get(key)
     if size is None:
         bytes_ = C.c_size_t()
-        call("prana_attention_tree_workspace", ctx, n_seq, max_nodes, n_heads, view.n_kv_heads, view.head_dim, C.byref(bytes_))
+        call("prana_attention_tree_workspace", ctx, max_nodes, n_heads, view.n_kv_heads, view.head_dim, C.byref(bytes_))
         size = _tree_work[key] = bytes_.value
     work = torch.empty(size, dtype=torch.uint8, device=device)  # of this stream: calls on other streams have their own
     call("prana_attention_tree", ctx, q.data_ptr(), C.byref(view), cache._int32(starts, (n_seq,), "starts"),

@@ -38,5 +38,5 @@ def test_null_arguments_are_codes():
     assert L.prana_kv_rows_read(None, C.byref(view), None, 1, 0, None, None) == INVALID
     assert L.prana_kv_rows_move(None, C.byref(view), None, None, None, None, 1, 1) == INVALID
     assert L.prana_attention_tree(None, None, C.byref(view), None, None, None, None, 1, 1, 1, 1, None, 0, None) == INVALID
-    assert L.prana_attention_tree_workspace(None, 1, 1, 1, 1, 64, C.byref(C.c_size_t())) == INVALID
+    assert L.prana_attention_tree_workspace(None, 1, 1, 1, 64, C.byref(C.c_size_t())) == INVALID
     assert b"null" in L.prana_last_error()
