@@ -265,6 +265,7 @@ __device__ __forceinline__ void tt_wait(uint64_t* bar, uint32_t phase, volatile 
   *abort = 1;
 }
 __device__ __forceinline__ void group_sync(int g) { asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory"); }
+__device__ __forceinline__ void first_sync() { asm volatile("bar.sync 6, 544;" ::: "memory"); }  // the groups and the column warp
 __device__ __forceinline__ void groups_sync() { asm volatile("bar.sync 5, 512;" ::: "memory"); }
 __device__ __forceinline__ bool groups_any(bool pred) {
   uint32_t r;
@@ -289,17 +290,27 @@ struct TreeWalk {
   int b, kvh, chunk, tile, tiles, chunks, group, ch;
   int left;  // tiles of the share still to go, this segment's included
   int seg;   // tiles of this segment
-  __device__ __forceinline__ void start(const TreeArgs* args, int ch_, int seq, unsigned long long at, int n) {
+  // tile `at` of sequence seq's work
+  __device__ __forceinline__ void start(const TreeArgs* args, int ch_, int seq, const TreeSeq& sq, unsigned long long at,
+                                        int n) {
     a = args;
     ch = ch_;
     group = a->n_heads / a->c.n_kv;
     b = seq;
     left = n;
-    load();
-    tile = (int)(at % tiles);
-    const unsigned long long u = at / tiles;
-    chunk = (int)(u % chunks);
-    kvh = (int)(u / chunks);
+    s = sq;
+    tiles = tree_tiles(s);
+    chunks = tree_chunks(s, group, ch);
+    unsigned long long u;
+    if (at <= 0xffffffffull) {
+      u = (unsigned)at / (unsigned)tiles;
+      kvh = (int)((unsigned)u / (unsigned)chunks);
+    } else {
+      u = at / tiles;
+      kvh = (int)(u / chunks);
+    }
+    tile = (int)(at - u * tiles);
+    chunk = (int)(u - (unsigned long long)kvh * chunks);
     seg = min(left, tiles - tile);
   }
   __device__ __forceinline__ void load() {
@@ -342,7 +353,12 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
   extern __shared__ __align__(16) uint8_t smem_dyn[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~(uintptr_t)1023);
   uint8_t* q_t = base + S::OFF_Q;
-  __shared__ __align__(8) uint64_t full[TT_MAX_SLOTS], empty[TT_MAX_SLOTS], s_full[4], s_free[4], p_full[4], o_full[4], q_ready, q_free, t_free, done_s, done_o;
+  // A waiter names a phase by its parity, so none may fall two phases behind: each
+  // barrier's next phase needs the waiter's own step past the last.  (K and V use
+  // a slot in turn when their number is odd, for two waiters: each has its own
+  // `full`.)
+  __shared__ __align__(8) uint64_t full[2][TT_MAX_SLOTS], empty[TT_MAX_SLOTS];  // full: of K, of V
+  __shared__ __align__(8) uint64_t s_full[4], s_free[4], p_full[4], o_full[4], q_ready, q_seen, q_free, done_s, done_o;
   __shared__ uint32_t tmem_s;
   __shared__ int s_abort;
   // a segment and its columns, in one of two sets: the nodes a column's node sees,
@@ -356,19 +372,22 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
   __shared__ __align__(16) float x_m[16][NQ], x_w[16][NQ], x_al[16][NQ], x_fold[16][2][NQ];  // per warp
   __shared__ float2 x_fin[4][NQ];              // (max, sum) of a finished segment
   __shared__ unsigned long long x_bad[4][2];   // drafted rows of V that are not finite
-  __shared__ unsigned long long w_sum[TT_THREADS / 32], s_total, s_at, s_all;
-  __shared__ int s_seq;
+  __shared__ unsigned long long w_sum[TT_THREADS / 32], s_total, s_all;
+  __shared__ TreeWalk s_walk;  // where the share begins
   volatile int* abort = &s_abort;
 
   const int tid = threadIdx.x, lane = tid & 31, wi = tid >> 5;
   const int hd = a.c.hd, n_kv = a.c.n_kv, group = a.n_heads / n_kv;
   const int slots = ta.slots, boxes = ta.boxes;
   const uint32_t slot_bytes = (uint32_t)boxes * 16384u;
+  const int period = slots & 1 ? slots : slots / 2;  // tiles between two uses of a slot by K (or by V)
 
   if (tid == 0) {
     s_abort = 0;
+    any_mask[0] = any_mask[1] = 0ull;
     for (int i = 0; i < slots; i++) {
-      mbar_init(&full[i], 1);
+      mbar_init(&full[0][i], 1);
+      mbar_init(&full[1][i], 1);
       mbar_init(&empty[i], 1);
     }
     for (int g = 0; g < TG; g++) {
@@ -379,7 +398,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
     }
     mbar_init(&q_ready, 32);
     mbar_init(&q_free, 1);
-    mbar_init(&t_free, TT_SOFT);
+    mbar_init(&q_seen, 1);
     mbar_init(&done_s, 1);
     mbar_init(&done_o, 1);
     fence_barrier_init();
@@ -394,53 +413,72 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
   // ---- this CTA's share of the tiles
   {
     const int n_seq = a.n_seq;
-    auto work = [&](int b) { return b < n_seq ? tree_work(tree_seq(a, b), n_kv, group, CH) : 0ull; };
-    const unsigned long long mine = work(tid);
-    unsigned long long sum = mine;
-    for (int b = tid + TT_THREADS; b < n_seq; b += TT_THREADS) sum += work(b);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) w_sum[wi] = sum;
-    __syncthreads();
-    unsigned long long total = 0;
-    for (int w = 0; w < TT_THREADS / 32; w++) total += w_sum[w];
     // no more shares than tiles, so that every share between two others holds something
-    const unsigned long long shares = total < gridDim.x ? total : gridDim.x;
-    const unsigned long long t0 = blockIdx.x < shares ? total * blockIdx.x / shares : total;
-    const unsigned long long t1 = blockIdx.x < shares ? total * (blockIdx.x + 1) / shares : total;
-    if (tid == 0) {
-      s_total = t1 - t0;
-      s_all = total;
-      s_seq = 0;
-      s_at = 0;
-      ta.parts[blockIdx.x].n = 0;
-    }
+    auto share = [&](unsigned long long total, unsigned i) {
+      const unsigned shares = total < gridDim.x ? (unsigned)total : gridDim.x;
+      if (i >= shares) return total;
+      return total <= 0xffffffull ? (unsigned long long)((unsigned)total * i / shares) : total * i / shares;
+    };
+    auto found = [&](const TreeSeq& sq, int b, unsigned long long at, unsigned long long n) {
+      s_walk.start(&a, CH, b, sq, at, (int)n);
+    };
     const bool all = blockIdx.x == 0;  // CTA 0 looks for sequences that do not fit
-    unsigned long long before = 0;
-    for (int b0 = 0; b0 < n_seq && (all || (t1 > t0 && before <= t0)); b0 += TT_THREADS) {
-      const int b = b0 + tid;
-      const unsigned long long w = b0 ? work(b) : mine;
-      unsigned long long inc = w;
+    auto look = [&](int b, const TreeSeq& sq) {
+      if (tree_seq_bad(a, b, sq)) atomicOr(a.err, ERR_RANGE);
+    };
+    auto scan = [&](unsigned long long x) {  // inclusive, over a warp
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long x = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += x;
+        const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
       }
+      return x;
+    };
+    if (tid == 0) ta.parts[blockIdx.x].n = 0;
+    if (n_seq <= 32) {  // one warp sees them all
+      if (wi == 0) {
+        TreeSeq sq{0, 0, 0, 0};
+        if (lane < n_seq) sq = tree_seq(a, lane);
+        const unsigned long long w = tree_work(sq, n_kv, group, CH), inc = scan(w);
+        const unsigned long long total = __shfl_sync(0xffffffffu, inc, 31);
+        const unsigned long long t0 = share(total, blockIdx.x), t1 = share(total, blockIdx.x + 1);
+        if (lane == 0) {
+          s_total = t1 - t0;
+          s_all = total;
+        }
+        if (w && inc - w <= t0 && t0 < inc && t1 > t0) found(sq, lane, t0 - (inc - w), t1 - t0);
+        if (all && lane < n_seq) look(lane, sq);
+      }
+    } else {
+      auto seq = [&](int b) { return b < n_seq ? tree_seq(a, b) : TreeSeq{0, 0, 0, 0}; };
+      unsigned long long sum = 0;
+      for (int b = tid; b < n_seq; b += TT_THREADS) sum += tree_work(seq(b), n_kv, group, CH);
+      sum = scan(sum);
+      if (lane == 31) w_sum[wi] = sum;
       __syncthreads();
-      if (lane == 31) w_sum[wi] = inc;
-      __syncthreads();
-      unsigned long long pre = before, chunk = 0;
-      for (int x = 0; x < TT_THREADS / 32; x++) {
-        if (x < wi) pre += w_sum[x];
-        chunk += w_sum[x];
+      unsigned long long total = 0;
+      for (int w = 0; w < TT_THREADS / 32; w++) total += w_sum[w];
+      const unsigned long long t0 = share(total, blockIdx.x), t1 = share(total, blockIdx.x + 1);
+      if (tid == 0) {
+        s_total = t1 - t0;
+        s_all = total;
       }
-      pre += inc - w;
-      if (w && pre <= t0 && t0 < pre + w) {
-        s_seq = b;
-        s_at = t0 - pre;
+      unsigned long long before = 0;
+      for (int b0 = 0; b0 < n_seq && (all || (t1 > t0 && before <= t0)); b0 += TT_THREADS) {
+        const int b = b0 + tid;
+        const TreeSeq sq = seq(b);
+        const unsigned long long w = tree_work(sq, n_kv, group, CH), inc = scan(w);
+        __syncthreads();
+        if (lane == 31) w_sum[wi] = inc;
+        __syncthreads();
+        unsigned long long pre = before + inc - w;
+        for (int x = 0; x < TT_THREADS / 32; x++) {
+          if (x < wi) pre += w_sum[x];
+          before += w_sum[x];
+        }
+        if (w && pre <= t0 && t0 < pre + w && t1 > t0) found(sq, b, t0 - pre, t1 - t0);
+        if (all && b < n_seq) look(b, sq);
       }
-      if (all && b < n_seq && tree_seq_bad(a, b, tree_seq(a, b))) atomicOr(a.err, ERR_RANGE);
-      before += chunk;
     }
   }
   tc_fence_before();
@@ -448,14 +486,94 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
   tc_fence_after();
   const uint32_t tmem = tmem_s;
   const int n_tiles = (int)s_total;
+  // A segment's columns: q operand, masks, places.  Eight lanes a column, four
+  // columns a warp at a time; this warp is number `at` of `warps`.
+  auto stage = [&](const TreeSegment& sg, int set, int at, int warps) {
+    const float scale2 = LOG2E / sqrtf((float)hd);
+    const int sub = lane & 7;
+    const TreeSeq sq{sg.row, sg.len, sg.total - sg.len, sg.off};
+#pragma unroll 1
+    for (int c = at * 4 + (lane >> 3); c < CH; c += warps * 4) {
+      const int vh = sg.vh0 + c, node = vh / group, head = sg.kvh * group + vh - node * group;
+      const bool in = c < sg.cols;
+      const int off = (node * a.n_heads + head) * hd;
+      const float* src = a.q + (size_t)sg.off * a.n_heads * hd + off;
+      float x[16], amax = 0.0f;
+      bool nan = false;
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        const int d = (e >> 2) * 32 + sub * 4 + (e & 3);
+        x[e] = in && d < hd ? src[d] : 0.0f;
+        nan |= x[e] != x[e];
+        amax = fmaxf(amax, fabsf(x[e]));
+      }
+      const unsigned long long mask = in ? tree_mask(a, sq, node) : 0ull;
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) {
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        nan |= __shfl_xor_sync(0xffffffffu, (int)nan, o) != 0;
+      }
+      float mul;
+      if constexpr (Q8) {
+        const float up = amax < 1e-25f ? 0x1p96f : 1.0f;  // keeps the quotient finite
+        const float inv = amax > 0.0f ? TT_DIGITS / (amax * up) : 0.0f;
+        mul = (amax / TT_DIGITS) * scale2;
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          uint32_t b[4];  // balanced digits, a byte each
+#pragma unroll
+          for (int z = 0; z < 4; z++)
+            b[z] = (uint32_t)(__float2int_rn(fminf(fmaxf(x[e + z] * up * inv, -TT_DIGITS), TT_DIGITS)) + 0x808080) ^ 0x808080u;
+#pragma unroll
+          for (int z = 0; z < 3; z++) {
+            const int row = z * CH + c, sh = 16 - 8 * z;
+            *reinterpret_cast<uint32_t*>(q_t + row * 128 + (((e / 2 + (sub >> 2)) ^ (row & 7)) << 4) + (sub & 3) * 4) =
+                (b[0] >> sh & 255u) | (b[1] >> sh & 255u) << 8 | (b[2] >> sh & 255u) << 16 | (b[3] >> sh & 255u) << 24;
+          }
+        }
+      } else {
+        // a power of two that brings the largest value to [2^13, 2^14)
+        const int e2 = amax > 0.0f && amax < INFINITY ? min(120, 13 - ilogbf(amax)) : 0;
+        const float up = __int_as_float((e2 + 127) << 23);
+        mul = scale2 / up;
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          alignas(8) __half hh[4], hl[4];
+#pragma unroll
+          for (int z = 0; z < 4; z++) {
+            const float v = x[e + z] * up;
+            hh[z] = __float2half_rn(v);
+            hl[z] = __float2half_rn(v - __half2float(hh[z]));
+          }
+#pragma unroll
+          for (int z = 0; z < 2; z++) {
+            const int row = z * CH + c, k = e * 8 + sub * 4;
+            *reinterpret_cast<uint2*>(q_t + (k >> 6) * (N * 128) + row * 128 + ((((k & 63) >> 3) ^ (row & 7)) << 4) + (k & 7) * 2) =
+                *reinterpret_cast<const uint2*>(z ? hl : hh);
+          }
+        }
+      }
+      if (sub == 0) {
+        col_off[set][c] = off;
+        col_mul[set][c] = nan ? __int_as_float(0x7fffffff) : mul;
+        col_mask[set][c] = mask;
+        if (!Q8 && mask) atomicOr(&any_mask[set], mask);
+      }
+    }
+    if constexpr (Q8 && NQ == 8) {  // the operand's last eight rows
+      if (at == 0)
+        for (int i = lane; i < 64; i += 32) *reinterpret_cast<uint4*>(q_t + 24 * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    fence_async_smem();
+  };
+
   // Team k % TG does the CTA's tile k, as its item k / TG.
   if (n_tiles == 0) {
     // nothing: fall through to the end
   } else if (wi == TT_TMA_WARP) {
     // ------------------------------------------------ TMA: K and V of every tile, slot after slot
     if (lane == 0) {
-      TreeWalk w;
-      w.start(&a, CH, s_seq, s_at, n_tiles);
+      TreeWalk w = s_walk;
       int slot = 0, used = 0;
       uint32_t phase = 1;  // a fresh barrier's previous phase counts as done
       bool go = true;
@@ -467,10 +585,10 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
               go = false;
               break;
             }
-            mbar_arrive_expect_tx(&full[slot], slot_bytes);
+            mbar_arrive_expect_tx(&full[kv][slot], slot_bytes);
             for (int x = 0; x < boxes; x++)
               tma_load_3d(base + slot * slot_bytes + x * 16384, kv ? &ta.tm_v : &ta.tm_k, x * 64, w.kvh,
-                          w.s.start + t * TT_TILE, &full[slot]);
+                          w.s.start + t * TT_TILE, &full[kv][slot]);
             used++;
             if (++slot == slots) {
               slot = 0;
@@ -480,19 +598,19 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
       } while (go && w.next());
       // wind down: every copy issued has landed before the CTA may exit
       for (int i = max(0, used - slots); i < used; i++)
-        if (!mbar_wait(&full[i % slots], (uint32_t)(i / slots) & 1, *abort ? 1u << 16 : kMbarPolls)) *abort = 1;
+        if (!mbar_wait(&full[i & 1][i % slots], (uint32_t)((i >> 1) / period) & 1, *abort ? 1u << 16 : kMbarPolls)) *abort = 1;
     }
     __syncwarp();
   } else if (wi == TT_S_WARP || wi == TT_O_WARP) {
     // ------------------------------------------------ MMA: scores (K slots), outputs (V slots)
     if (lane == 0) {
-      TreeWalk w;
-      w.start(&a, CH, s_seq, s_at, n_tiles);
+      TreeWalk w = s_walk;
       const bool scores = wi == TT_S_WARP;
       const int ks_n = Q8 ? (hd + 31) / 32 : (hd + 15) / 16;
       constexpr uint32_t IDESC_S = tt_idesc<Q8>(N, false), IDESC_O = tt_idesc<Q8>(N, true);
       int slot = scores ? 0 : 1, seg_left = w.seg;
       uint32_t phase = 0, segs = 0;
+      int turn = 0;  // of `period` tiles, after which a slot's barrier is in its next phase
       bool fresh = true;  // a segment begins: its columns first
       for (int k = 0; k < n_tiles && !*abort; k++) {
         const int g = k % TG;
@@ -500,7 +618,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
         if (scores) {
           if (fresh) tt_wait(&q_ready, segs & 1, abort);
           if (n) tt_wait(&s_free[g], (n - 1) & 1, abort);
-          tt_wait(&full[slot], phase, abort);
+          tt_wait(&full[scores ? 0 : 1][slot], phase, abort);
           if (*abort) break;
           tc_fence_after();
           const uint64_t kd = sw128_desc(smem_u32(base + slot * slot_bytes));
@@ -526,7 +644,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
           }
         } else {
           tt_wait(&p_full[g], n & 1, abort);
-          tt_wait(&full[slot], phase, abort);
+          tt_wait(&full[scores ? 0 : 1][slot], phase, abort);
           if (*abort) break;
           tc_fence_after();
           // one 128-byte-wide block of M per box; a lone f16 box stands for both
@@ -545,8 +663,9 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
         }
         tc_commit(&empty[slot]);
         slot += 2;  // K and V alternate
-        if (slot >= slots) {
-          slot -= slots;
+        if (slot >= slots) slot -= slots;
+        if (++turn == period) {
+          turn = 0;
           phase ^= 1;
         }
       }
@@ -558,100 +677,28 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
     __syncwarp();
   } else if (wi == TT_Q_WARP) {
     // ------------------------------------------------ the next segment's columns: q operand, masks, places
-    const float scale2 = LOG2E / sqrtf((float)hd);
-    TreeWalk w;
-    w.start(&a, CH, s_seq, s_at, n_tiles);
+    TreeWalk w = s_walk;
     int seg = 0;
     bool more;
     do {
       const int set = seg & 1, cols = min(CH, w.s.n * group - w.chunk * CH);
-      const float* q_seq = a.q + (size_t)w.s.off * a.n_heads * hd;
-      if (seg >= 2) tt_wait(&t_free, (uint32_t)seg & 1, abort);  // the set's readers, two segments ago
+      // everybody is in the last segment, so the set's readers, two segments ago, are done
+      if (seg) tt_wait(&q_seen, (uint32_t)(seg - 1) & 1, abort);
       if (*abort) break;
       TreeSegment sg{w.s.start + w.tile * TT_TILE, w.s.len - w.tile * TT_TILE, w.s.len + w.s.n - w.tile * TT_TILE, w.s.off,
                      w.kvh, w.seg, w.tile == 0, w.tiles - w.tile - w.seg, w.chunk * CH, cols, 0};
-      if (lane == 0) any_mask[set] = 0ull;
-      bool q_mine = seg == 0;
-      for (int cb = 0; cb < CH; cb += 4) {
-        float x[4][4];
-        unsigned long long mask[4];
-#pragma unroll
-        for (int u = 0; u < 4; u++) {  // four columns' loads at once
-          const int vh = w.chunk * CH + cb + u, node = vh / group, head = w.kvh * group + vh % group;
-          const bool in = cb + u < cols;
-          const int off = (node * a.n_heads + head) * hd;
-          mask[u] = in ? tree_mask(a, w.s, node) : 0ull;
-          if (lane == 0) col_off[set][cb + u] = off;
-#pragma unroll
-          for (int e = 0; e < 4; e++) x[u][e] = in && lane * 4 + e < hd ? q_seq[off + lane * 4 + e] : 0.0f;
-        }
-        if (!q_mine) {  // the last segment's products have read the operand
-          tt_wait(&q_free, (uint32_t)(seg - 1) & 1, abort);
-          q_mine = true;
-        }
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-          const int c = cb + u;
-          float amax = 0.0f;
-          bool nan = false;
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            nan |= x[u][e] != x[u][e];
-            amax = fmaxf(amax, fabsf(x[u][e]));
-          }
-          amax = redux_max(amax);
-          nan = __any_sync(0xffffffffu, nan);
-          float mul;
-          if constexpr (Q8) {
-            const float up = amax < 1e-25f ? 0x1p96f : 1.0f;  // keeps the quotient finite
-            const float inv = amax > 0.0f ? TT_DIGITS / (amax * up) : 0.0f;
-            mul = (amax / TT_DIGITS) * scale2;
-            uint32_t dig[3] = {0u, 0u, 0u};
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-              const int v = __float2int_rn(fminf(fmaxf(x[u][e] * up * inv, -TT_DIGITS), TT_DIGITS));
-              const uint32_t b = (uint32_t)(v + 0x808080) ^ 0x808080u;  // balanced digits, a byte each
-#pragma unroll
-              for (int z = 0; z < 3; z++) dig[z] |= (b >> (16 - 8 * z) & 255u) << (8 * e);
-            }
-#pragma unroll
-            for (int z = 0; z < 3; z++) {
-              const int row = z * CH + c;
-              *reinterpret_cast<uint32_t*>(q_t + row * 128 + (((lane >> 2) ^ (row & 7)) << 4) + (lane & 3) * 4) = dig[z];
-            }
-          } else {
-            // a power of two that brings the largest value to [2^13, 2^14)
-            const int e2 = amax > 0.0f && amax < INFINITY ? min(120, 13 - ilogbf(amax)) : 0;
-            const float up = __int_as_float((e2 + 127) << 23);
-            mul = scale2 / up;
-            alignas(8) __half hh[4], hl[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-              const float v = x[u][e] * up;
-              hh[e] = __float2half_rn(v);
-              hl[e] = __float2half_rn(v - __half2float(hh[e]));
-            }
-#pragma unroll
-            for (int z = 0; z < 2; z++) {
-              const int row = z * CH + c, k = lane * 4;
-              *reinterpret_cast<uint2*>(q_t + (k >> 6) * (N * 128) + row * 128 + ((((k & 63) >> 3) ^ (row & 7)) << 4) + (k & 7) * 2) =
-                  *reinterpret_cast<const uint2*>(z ? hl : hh);
-            }
-          }
-          if (lane == 0) {
-            col_mul[set][c] = nan ? __int_as_float(0x7fffffff) : mul;
-            col_mask[set][c] = mask[u];
-            any_mask[set] |= mask[u];
-          }
-        }
-      }
-      if constexpr (Q8 && NQ == 8) {  // the operand's last eight rows
-        for (int i = lane; i < 64; i += 32) *reinterpret_cast<uint4*>(q_t + 24 * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+      if (seg) {
+        tt_wait(&q_free, (uint32_t)(seg - 1) & 1, abort);  // the last segment's products have read the operand
+        stage(sg, set, 0, 1);
+      } else {
+        if (lane == 0) seg_tab[0] = sg;
+        first_sync();
+        stage(sg, 0, TT_SOFT / 32, TT_SOFT / 32 + 1);
+        first_sync();
       }
       more = w.next();
       sg.more = more;
       if (lane == 0) seg_tab[set] = sg;
-      fence_async_smem();
       mbar_arrive(&q_ready);
       seg++;
     } while (more && !*abort);
@@ -666,12 +713,17 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
     int item = 0;  // of this group, over all segments
     int k0 = 0;    // tiles of the CTA before this segment
     int seg_no = 0, more;
+    // the first segment's columns are everybody's work
+    first_sync();
+    stage(seg_tab[0], 0, wi, TT_SOFT / 32 + 1);
+    first_sync();
     do {
       const int set = seg_no & 1;
       tt_wait(&q_ready, (uint32_t)seg_no & 1, abort);  // the segment and its columns' tables
       // one decision for all, so that the named barriers stay matched; from here
       // on the last segment's p operands are free
       if (groups_any(*abort != 0)) break;
+      if (tid == 0) mbar_arrive(&q_seen);
       const TreeSegment& sg = seg_tab[set];
       const int len = sg.len, total = sg.total, tiles = sg.tiles;
       const int first = (tg - k0) & (TG - 1);
@@ -912,11 +964,11 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
           }
           // V of places nobody sees, and values that are not finite in drafted rows, become zeros
           if (edge) {
-            const int v_no = 2 * (k0 + t) + 1;  // K and V alternate over the CTA's tiles
+            const int v_slot = (2 * (k0 + t) + 1) % slots;  // K and V alternate over the CTA's tiles
             const bool row_gone = j >= 0 && !(there && (any_mask[set] >> j & 1));
             if (row_gone || odd) {
-              tt_wait(&full[v_no % slots], (uint32_t)(v_no / slots) & 1, abort);
-              uint8_t* vt = base + (v_no % slots) * slot_bytes + r * 128;
+              tt_wait(&full[1][v_slot], (uint32_t)((k0 + t) / period) & 1, abort);
+              uint8_t* vt = base + v_slot * slot_bytes + r * 128;
               for (int c = 0; c < 8 * boxes; c++)
                 if (row_gone || (odd >> c & 1)) {
                   uint4* at = reinterpret_cast<uint4*>(vt + (c >> 3) * 16384 + (((c & 7) ^ (r & 7)) << 4));
@@ -1006,7 +1058,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
         }
       }
       more = sg.more;
-      mbar_arrive(&t_free);
+      if (!Q8 && tid == 0) any_mask[set] = 0ull;
       k0 += tiles;
       seg_no++;
     } while (more);

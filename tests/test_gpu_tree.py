@@ -287,6 +287,19 @@ def test_the_same_bits_every_time_and_on_any_stream(gpu, kind):
 
 
 @pytest.mark.parametrize("kind", ["q8", "f16"])
+@pytest.mark.parametrize("heads,lens,nodes", [((32, 8, 128), [9000, 1, 4000, 130, 7000] * 3, [1] * 15), ((32, 8, 128), [3000, 129, 600] * 4, [20, 1, 60] * 4),
+                                              ((14, 2, 64), [40, 3, 300, 90] * 50, [2, 5, 1, 9] * 50)])
+def test_many_runs_give_one_answer(gpu, kind, heads, lens, nodes):
+    """Long and short units side by side in every share, over and over: no wait runs out, no tile is taken for another."""
+    b = Batch(kind, *heads, lens=lens, nodes=nodes)
+    want = b.run().clone()
+    for _ in range(60):
+        assert torch.equal(b.run(), want)
+    K.synchronize()
+    b.check(want)
+
+
+@pytest.mark.parametrize("kind", ["q8", "f16"])
 def test_captured_into_a_graph(gpu, kind):
     b = Batch(kind, 8, 2, 128, lens=[500, 40], nodes=[5, 5])
     want = b.run().clone()
