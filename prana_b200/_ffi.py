@@ -170,5 +170,13 @@ def check(rc: int) -> None:
         raise PranaError(rc, lib().prana_last_error().decode(errors="replace"))
 
 
+_fns: dict = {}
+
+
 def call(name: str, *args) -> None:
-    check(getattr(lib(), name)(*args))
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(lib(), name)
+    rc = fn(*args)
+    if rc != PRANA_OK:
+        check(rc)

@@ -720,6 +720,7 @@ int prana_attention_tree(prana_ctx* c, const float* q, const prana_kv_rows* cach
   a.out = out;
   a.err = c->err;
   a.sm_count = c->sm_count;
+  a.device = c->device;
   PRANA_CK(launch_attn_tree(a, c->stream));
   return PRANA_OK;
 }

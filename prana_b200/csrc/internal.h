@@ -228,7 +228,7 @@ struct TreeArgs {
   float* out;  // [n_nodes][n_heads * hd]
   void* work;
   unsigned* err;
-  int sm_count;
+  int sm_count, device;
 };
 // tensor map of cache rows (attention.cu); false: their strides or alignment do not take one
 bool encode_rows_map(CUtensorMap* m, const void* base, bool q8, int positions, int n_kv, int hd, size_t row_stride,

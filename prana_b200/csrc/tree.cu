@@ -5,6 +5,8 @@
 //   s_j = q . k_j / sqrt(hd) over the context and the nodes in its mask,
 //   out = sum_j exp(s_j - max) v_j / sum_j exp(s_j - max)   (zeros: nothing seen)
 // A place that a node does not see takes no part, whatever it holds.
+#include <atomic>
+
 #include "internal.h"
 #include "mbar.cuh"
 #include "tc.cuh"
@@ -1139,8 +1141,14 @@ template <bool Q8, int NQ, int CG>
 static cudaError_t tt_go(TreeTcArgs& ta, cudaStream_t st) {
   using S = TtShape<Q8, NQ, CG>;
   auto k = tree_tc_kernel<Q8, NQ, CG>;
-  cudaError_t e = cudaFuncSetAttribute((const void*)k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::BYTES);
-  if (e != cudaSuccess) return e;
+  static std::atomic<unsigned long long> ready{0};  // devices this kernel has its shared memory on
+  const unsigned long long dev = 1ull << (ta.t.device & 63);
+  cudaError_t e = cudaSuccess;
+  if (!(ready.load(std::memory_order_relaxed) & dev)) {
+    e = cudaFuncSetAttribute((const void*)k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::BYTES);
+    if (e != cudaSuccess) return e;
+    ready.fetch_or(dev, std::memory_order_relaxed);
+  }
   ta.slots = S::RING / (ta.boxes * 16384);
   if (ta.slots > TT_MAX_SLOTS) ta.slots = TT_MAX_SLOTS;
   void* args[] = {&ta};

@@ -22,7 +22,10 @@ QK_K = 256
 BLOCK_BYTES = {TYPE_Q8_0: (32, 34), TYPE_Q4_0: (32, 18), TYPE_Q4_K: (256, 144), TYPE_Q6_K: (256, 210)}
 
 _ctxs: dict[int, C.c_void_p] = {}
-_tree_work: dict[tuple, int] = {}  # workspace bytes of attention_tree by sizes
+# attention_tree's workspaces by (device, stream): calls on one stream follow one another
+_tree_work: dict[tuple, torch.Tensor] = {}
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle, without a Stream object
+_capturing = torch._C._cuda_isCurrentStreamCapturing
 
 
 def context(device: int | None = None) -> C.c_void_p:
@@ -36,8 +39,7 @@ def context(device: int | None = None) -> C.c_void_p:
         _ctxs[device] = ctx
     # torch reports its legacy default stream as handle 0; the ABI's NULL means
     # "the context's own stream", so pass cudaStreamLegacy (0x1) explicitly.
-    handle = torch.cuda.current_stream(device).cuda_stream or 1
-    call("prana_ctx_set_stream", ctx, C.c_void_p(handle))
+    call("prana_ctx_set_stream", ctx, _raw_stream(device) or 1)
     return ctx
 
 
@@ -332,39 +334,41 @@ class KvRows:
     and v (and the two scales) are laid out alike.  The rows of many sequences
     may share one KvRows."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "quantized", "_view")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "quantized", "device", "n_kv_heads", "head_dim", "_view", "_ref")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None,
                  v_scale: torch.Tensor | None = None):
-        shape, strides = k.shape, k.stride()
-        if len(shape) != 3 or v.shape != shape or v.stride() != strides or v.dtype != k.dtype:
+        shape, strides, device, dtype = k.shape, k.stride(), k.device, k.dtype
+        if len(shape) != 3 or v.shape != shape or v.stride() != strides or v.dtype != dtype:
             raise ValueError("k and v must be [positions, n_kv_heads, head_dim] of one type and layout")
-        if strides[2] != 1 and shape[2] != 1:
+        positions, n_kv, hd = shape
+        if strides[2] != 1 and hd != 1:
             raise ValueError("the head dimension must be contiguous")
-        device = k.device
-        if device.type != "cuda" or v.device != device:
+        if not k.is_cuda or v.device != device:
             raise ValueError("expected CUDA tensors of one device")
-        self.quantized = k.dtype == torch.int8
-        scale_strides = (0, 0)
-        if self.quantized:
+        if dtype == torch.int8:
             if k_scale is None or v_scale is None:
                 raise ValueError("an int8 cache needs k_scale and v_scale")
-            scale_strides = k_scale.stride()
-            if k_scale.shape != shape[:2] or v_scale.shape != shape[:2] or v_scale.stride() != scale_strides:
+            scale_strides, scale_shape = k_scale.stride(), k_scale.shape
+            if scale_shape != (positions, n_kv) or v_scale.shape != scale_shape or v_scale.stride() != scale_strides:
                 raise ValueError("scales must be [positions, n_kv_heads] of one layout")
             if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
                 raise TypeError("scales must be float32")
             if k_scale.device != device or v_scale.device != device:
                 raise ValueError("expected CUDA tensors of one device")
-        elif k.dtype != torch.float16:
+            self.quantized = True
+            self._view = view = _ffi.KvRowsView(_ffi.KV_Q8, k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                                                positions, n_kv, hd, strides[0], strides[1], scale_strides[0], scale_strides[1])
+        elif dtype != torch.float16:
             raise TypeError("a cache holds float16 or int8")
         elif k_scale is not None or v_scale is not None:
             raise ValueError("a float16 cache has no scales")
+        else:
+            self.quantized = False
+            self._view = view = _ffi.KvRowsView(_ffi.KV_F16, k.data_ptr(), v.data_ptr(), None, None, positions, n_kv, hd,
+                                                strides[0], strides[1], 0, 0)
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self._view = _ffi.KvRowsView(
-            _ffi.KV_Q8 if self.quantized else _ffi.KV_F16, k.data_ptr(), v.data_ptr(),
-            k_scale.data_ptr() if self.quantized else None, v_scale.data_ptr() if self.quantized else None,
-            shape[0], shape[1], shape[2], strides[0], strides[1], scale_strides[0], scale_strides[1])
+        self.device, self.n_kv_heads, self.head_dim, self._ref = device, n_kv, hd, C.byref(view)
 
     @classmethod
     def alloc(cls, positions: int, n_kv_heads: int, head_dim: int, quantized: bool = True,
@@ -383,7 +387,7 @@ class KvRows:
             raise TypeError(f"{what} must be int32")
         if t.shape != shape:
             raise ValueError(f"{what} must have shape {list(shape)}")
-        if t.device != self.k.device or not t.is_contiguous():
+        if t.device != self.device or not t.is_contiguous():
             raise ValueError(f"{what} must be a contiguous tensor on the cache's device")
         return t.data_ptr()
 
@@ -392,19 +396,19 @@ def kv_rows_write(cache: KvRows, rows: torch.Tensor, k: torch.Tensor, v: torch.T
     """Cache row rows[i] (int32; negative: skipped) = row i of k and v, [n, n_kv_heads,
     head_dim] or [n, n_kv_heads * head_dim] in float32 or float16.  An int8 cache
     quantises each head row as it is written: scale = amax / 127, as quantize_q8."""
-    view = cache._view
-    n, width = rows.numel(), view.n_kv_heads * view.head_dim
-    if k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.numel() != n * width:
+    n, device = rows.numel(), cache.device
+    width = cache.n_kv_heads * cache.head_dim
+    dtype, shape, strides = k.dtype, k.shape, k.stride()
+    if v.shape != shape or v.stride() != strides or v.dtype != dtype or k.numel() != n * width or len(shape) < 2 or shape[0] != n:
         raise ValueError("k and v must hold one cache row for each index, laid out alike")
-    if k.dtype not in _SRC_TYPES:
+    if dtype not in _SRC_TYPES:
         raise TypeError("k and v must be float32 or float16")
-    if k.device != cache.k.device or v.device != cache.k.device:
+    if k.device != device or v.device != device:
         raise ValueError("k and v must be on the cache's device")
-    stride = k.stride(0) if n else 0
-    if n and not k[0].is_contiguous():
+    if n and not k.is_contiguous() and not k[0].is_contiguous():
         raise ValueError("a row of k and v must be contiguous")
-    call("prana_kv_rows_write", context(cache.k.device.index), C.byref(view), cache._int32(rows, (n,), "rows"), n,
-         _SRC_TYPES[k.dtype], k.data_ptr(), v.data_ptr(), stride)
+    call("prana_kv_rows_write", context(device.index), cache._ref, cache._int32(rows, (n,), "rows"), n,
+         _SRC_TYPES[dtype], k.data_ptr(), v.data_ptr(), strides[0])
 
 
 def kv_rows_read(cache: KvRows, rows: torch.Tensor, dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
@@ -412,23 +416,21 @@ def kv_rows_read(cache: KvRows, rows: torch.Tensor, dtype: torch.dtype = torch.f
     [n, n_kv_heads, head_dim] in float32 or float16."""
     if dtype not in _SRC_TYPES:
         raise TypeError("rows are read as float32 or float16")
-    view, n = cache._view, rows.numel()
-    out = torch.empty((2, n, view.n_kv_heads, view.head_dim), dtype=dtype, device=cache.k.device)
-    k, v = out.unbind(0)
-    call("prana_kv_rows_read", context(cache.k.device.index), C.byref(view), cache._int32(rows, (n,), "rows"), n,
-         _SRC_TYPES[dtype], k.data_ptr(), v.data_ptr())
+    n, device = rows.numel(), cache.device
+    k, v = torch.empty((2, n, cache.n_kv_heads, cache.head_dim), dtype=dtype, device=device).unbind(0)
+    call("prana_kv_rows_read", context(device.index), cache._ref, cache._int32(rows, (n,), "rows"), n, _SRC_TYPES[dtype],
+         k.data_ptr(), v.data_ptr())
     return k, v
 
 
 def kv_rows_move(cache: KvRows, starts: torch.Tensor, lens: torch.Tensor, path: torch.Tensor, counts: torch.Tensor) -> None:
     """Close accepted branches up: for i < counts[b], row starts[b] + lens[b] + i becomes
     what row starts[b] + lens[b] + path[b, i] was.  path is int32 [n_seq, at most 64]."""
-    n = starts.numel()
-    if path.dim() != 2:
+    n, shape = (starts.numel(),), path.shape
+    if len(shape) != 2 or shape[0] != n[0]:
         raise ValueError("path must be [n_seq, nodes]")
-    call("prana_kv_rows_move", context(cache.k.device.index), C.byref(cache._view), cache._int32(starts, (n,), "starts"),
-         cache._int32(lens, (n,), "lens"), cache._int32(path, (n, path.shape[1]), "path"),
-         cache._int32(counts, (n,), "counts"), n, path.shape[1])
+    call("prana_kv_rows_move", context(cache.device.index), cache._ref, cache._int32(starts, n, "starts"),
+         cache._int32(lens, n, "lens"), cache._int32(path, shape, "path"), cache._int32(counts, n, "counts"), n[0], shape[1])
 
 
 def tree_masks(parents) -> list[int]:
@@ -455,9 +457,8 @@ def attention_tree(q: torch.Tensor, cache: KvRows, starts: torch.Tensor, lens: t
     nodes whose bits are set in its mask (int64 [n_nodes], see tree_masks; None:
     itself and the nodes before it).  With one node per sequence this is
     attention_decode for a batch.  starts, lens, offsets are int32."""
-    view, n_seq, n_nodes = cache._view, starts.numel(), q.shape[0]
-    device = cache.k.device
-    width = n_heads * view.head_dim
+    n_seq, n_nodes, device = starts.numel(), q.shape[0], cache.device
+    width = n_heads * cache.head_dim
     if q.dtype != torch.float32 or q.device != device or not q.is_contiguous() or q.numel() != n_nodes * width:
         raise ValueError("q must be a contiguous float32 [n_nodes, n_heads * head_dim] on the cache's device")
     mask_ptr = None
@@ -469,17 +470,19 @@ def attention_tree(q: torch.Tensor, cache: KvRows, starts: torch.Tensor, lens: t
         out = torch.empty((n_nodes, width), dtype=torch.float32, device=device)
     elif out.dtype != torch.float32 or out.device != device or not out.is_contiguous() or out.numel() != n_nodes * width:
         raise ValueError("out must be a contiguous float32 [n_nodes, n_heads * head_dim] on the cache's device")
-    ctx = context(device.index)
-    key = (device.index, max_nodes, n_heads, view.n_kv_heads, view.head_dim)
-    size = _tree_work.get(key)
-    if size is None:
-        bytes_ = C.c_size_t()
-        call("prana_attention_tree_workspace", ctx, max_nodes, n_heads, view.n_kv_heads, view.head_dim, C.byref(bytes_))
-        size = _tree_work[key] = bytes_.value
-    work = torch.empty(size, dtype=torch.uint8, device=device)  # of this stream: calls on other streams have their own
-    call("prana_attention_tree", ctx, q.data_ptr(), C.byref(view), cache._int32(starts, (n_seq,), "starts"),
+    index = device.index
+    ctx = context(index)
+    size = C.c_size_t()
+    call("prana_attention_tree_workspace", ctx, max_nodes, n_heads, cache.n_kv_heads, cache.head_dim, C.byref(size))
+    key = (index, _raw_stream(index))
+    work = _tree_work.get(key)
+    if work is None or work.numel() < size.value or _capturing():
+        work = torch.empty(size.value, dtype=torch.uint8, device=device)
+        if not _capturing():  # a graph's memory belongs to the graph
+            _tree_work[key] = work
+    call("prana_attention_tree", ctx, q.data_ptr(), cache._ref, cache._int32(starts, (n_seq,), "starts"),
          cache._int32(lens, (n_seq,), "lens"), cache._int32(offsets, (n_seq + 1,), "offsets"), mask_ptr, n_seq, n_nodes,
-         max_nodes, n_heads, work.data_ptr(), size, out.data_ptr())
+         max_nodes, n_heads, work.data_ptr(), work.numel(), out.data_ptr())
     return out
 
 
