@@ -110,16 +110,19 @@ __global__ void __launch_bounds__(TR_THREADS) tree_simple_kernel(const TreeArgs 
 // there; otherwise its shares leave (max, sum, o) partials for tree_merge_kernel.
 //
 // Exactness.  An f16 cache: q and p enter as f16 head + remainder pairs (22
-// bits), K and V as they are.  An int8 cache: q and p as three signed base-256
-// digits (23 bits) and kind::i8 products, so K and V enter as they lie in memory
-// with no conversion, and every product and sum is an exact integer; a digit's
-// sum stays below 2^22 (128 x 128 x 128).  The K scale multiplies the score in
-// f32.  The V scale, 2^e * m, goes with the probability: e is added to the score
-// (in powers of two), so that p * 2^e of a tile is taken against its own largest
-// value, and m scales the digits.  The fixed point is then as fine as what the
-// tile adds to the output needs: against a running maximum of the scores alone,
-// 10^5 places of 2^-26 beside one large score with a small value would all round
-// to nothing.
+// bits), K and V as they are, sums in f32.  An int8 cache: q enters as three signed
+// base-256 digits (23 bits), p as four (31), and kind::i8 products take K and V as
+// they lie in memory, with no conversion; every product and sum is an exact
+// integer (a digit's sum over a tile stays within 2^21).  The K scale multiplies
+// the score in f32.  The V scale, 2^e * m, goes with the probability: e is added to
+// the score (in powers of two), so that p * 2^e, what the place adds to the
+// output, is measured against a reference of the same kind, and m scales the
+// digits.
+//   The reference of a column is its largest score when it was last set; it
+// is set at the first tile, at tiles with drafted places, and when a later score
+// passes it by more than TT_ROOM powers of two, which the digits and the f16 range
+// have to spare (p = 1 keeps 26 bits).  Until then O gathers in TMEM over the
+// tiles, and a tile needs no maximum, no exchange and no rescaling.
 //
 // Roles (20 warps): 16 loads K and V tiles by TMA into a ring of slots, 17 issues
 // S = K . q^T (M = 128 positions), 18 issues O^T = V^T . p^T (M = dims; V is read
@@ -136,7 +139,13 @@ constexpr int TT_TMA_WARP = 16, TT_S_WARP = 17, TT_O_WARP = 18, TT_Q_WARP = 19;
 constexpr int TT_TILE = 128;
 constexpr int TT_MAX_SLOTS = 10;
 constexpr float TT_DIGITS = 8355711.0f;  // 0x7f7f7f: the largest value of three balanced digits
-constexpr float TT_BIAS = 8421504.0f;    // 2^23 + 0x8080: rounds to an integer whose bytes are the digits, two of them + 128
+constexpr float TT_ROOM = 8.0f;
+// Units of the p operand for p = 1 (with m < 2): 2^4 * 2 of them stay below
+// 0x7f7f7f7f, the largest value of four digits, 2^4 * 2^11 below f16's largest.
+template <bool Q8>
+constexpr float TT_UNITS = Q8 ? 2139000000.0f / 512.0f : 128.0f;
+// Tiles that O may gather: 2^21 x 512 fits 32 bits
+constexpr int TT_RUN = 512;
 constexpr float LOG2E = 1.4426950408889634f;
 
 // What a CTA leaves for the merge: the unit that began in it and went on in
@@ -159,16 +168,18 @@ template <bool Q8, int NQ, int CG>
 struct TtShape {
   static constexpr int CH = NQ * CG;                               // columns of a CTA
   static constexpr int TG = TT_GROUPS / CG;                        // teams: tiles in work at once
-  static constexpr int N = Q8 ? (NQ == 8 ? 32 : 3 * CH) : 2 * CH;  // MMA columns: digit by digit, or heads and remainders
-  static constexpr int CS = (N + 31) / 32 * 32;                    // TMEM columns between accumulators
-  static constexpr int TMEM = 2 * TG * CS <= 128 ? 128 : 2 * TG * CS <= 256 ? 256 : 512;
-  static constexpr int QSZ = N * (Q8 ? 128 : 256);                 // bytes of the q operand
-  static constexpr int BLOCKS = (N * (Q8 ? 1 : 2) + 63) / 64;      // 64-byte blocks of a p row
-  static constexpr int PBLOCK = TT_TILE * 64, PSZ = BLOCKS * PBLOCK;  // bytes of a block, of a team's p operand
-  static constexpr int RING = (CG < 4 ? 160 : Q8 ? 144 : 128) * 1024;
+  // MMA columns of S and O: digit by digit, or heads and remainders
+  static constexpr int N = Q8 ? (NQ == 8 ? 32 : 3 * CH) : 2 * CH, NO = Q8 ? 4 * CH : 2 * CH;
+  static constexpr int CS = (N + 31) / 32 * 32, CO = (NO + 31) / 32 * 32;  // TMEM columns between accumulators
+  static constexpr int TMEM = TG * (CS + CO) <= 128 ? 128 : TG * (CS + CO) <= 256 ? 256 : 512;
+  static constexpr int QSZ = N * (Q8 ? 128 : 256);                  // bytes of the q operand
+  static constexpr int PSZ = (4 * CH + 63) / 64 * TT_TILE * 64;     // of a team's p operand: blocks of 64 bytes a position
+  static constexpr int RING = (CG < 4 ? 160 : 128) * 1024;
   static constexpr int OFF_P = RING, OFF_Q = OFF_P + TG * PSZ;
   static constexpr size_t BYTES = 1024 + OFF_Q + QSZ;
-  static_assert(2 * TG * CS <= 512, "TMEM");
+  static_assert(TG * (CS + CO) <= 512, "TMEM");
+  // a segment's start and end, in tiles (8 to 14 thousand cycles against 1.5 of a decode tile, 4 of a wide one)
+  static constexpr int LEAD = CG == 1 ? 4 : 2;
   static_assert(TG == 1 || PSZ >= CG * NQ * 128 * 4, "the groups' o pass through the p operand");
 };
 
@@ -197,38 +208,20 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// pairs of floats, one instruction for both
+// Two columns.  (The packed f32x2 instructions were slower here: they take no
+// constants as operands, and the moves that bring those into register pairs cost
+// more than the packing saves.)
 struct F2 {
-  unsigned long long v;
+  float x, y;
   __device__ __forceinline__ F2() {}
-  __device__ __forceinline__ F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
-  __device__ __forceinline__ explicit F2(float a) : F2(a, a) {}
-  __device__ __forceinline__ float lo() const {
-    float a, b;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-    return a;
-  }
-  __device__ __forceinline__ float hi() const {
-    float a, b;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-    return b;
-  }
+  __device__ __forceinline__ F2(float a, float b) : x(a), y(b) {}
+  __device__ __forceinline__ explicit F2(float a) : x(a), y(a) {}
+  __device__ __forceinline__ float lo() const { return x; }
+  __device__ __forceinline__ float hi() const { return y; }
 };
-__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
-  F2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) { return F2(a.x + b.x, a.y + b.y); }
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) { return F2(a.x * b.x, a.y * b.y); }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) { return F2(fmaf(a.x, b.x, c.x), fmaf(a.y, b.y, c.y)); }
 // two integers in [-2^22, 2^22) as floats, without the conversion unit
 __device__ __forceinline__ F2 small_ints(uint32_t a, uint32_t b) {
   return F2(__uint_as_float(a + 0x4B400000u), __uint_as_float(b + 0x4B400000u)) + F2(-12582912.0f);
@@ -267,6 +260,17 @@ __device__ __forceinline__ void tt_wait(uint64_t* bar, uint32_t phase, volatile 
   *abort = 1;
 }
 __device__ __forceinline__ void group_sync(int g) { asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory"); }
+// the OR of `pred` over the 128 * N threads of a team (barriers 7 and up)
+template <int N>
+__device__ __forceinline__ bool team_any(int team, bool pred) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.or.pred q, %2, %3, p;\n selp.u32 %0, 1, 0, q;\n}"
+      : "=r"(r)
+      : "r"((uint32_t)pred), "r"(7 + team), "n"(128 * N)
+      : "memory");
+  return r != 0;
+}
 __device__ __forceinline__ void first_sync() { asm volatile("bar.sync 6, 544;" ::: "memory"); }  // the groups and the column warp
 __device__ __forceinline__ void groups_sync() { asm volatile("bar.sync 5, 512;" ::: "memory"); }
 __device__ __forceinline__ bool groups_any(bool pred) {
@@ -281,59 +285,64 @@ __device__ __forceinline__ bool groups_any(bool pred) {
 
 __device__ __forceinline__ int tree_tiles(const TreeSeq& s) { return (s.len + s.n + TT_TILE - 1) / TT_TILE; }
 __device__ __forceinline__ int tree_chunks(const TreeSeq& s, int group, int ch) { return (s.n * group + ch - 1) / ch; }
-__device__ __forceinline__ unsigned long long tree_work(const TreeSeq& s, int n_kv, int group, int ch) {
-  return s.n ? (unsigned long long)tree_tiles(s) * tree_chunks(s, group, ch) * n_kv : 0ull;
+// A unit counts as its tiles and `lead` more in front, which stand for what
+// beginning and ending it costs; a share that ends among those has none of it.
+__device__ __forceinline__ unsigned long long tree_work(const TreeSeq& s, int n_kv, int group, int ch, int lead) {
+  return s.n ? (unsigned long long)(tree_tiles(s) + lead) * tree_chunks(s, group, ch) * n_kv : 0ull;
 }
 
 // A CTA's walk over its share: segments of consecutive tiles of one unit.
 struct TreeWalk {
   const TreeArgs* a;
   TreeSeq s;
-  int b, kvh, chunk, tile, tiles, chunks, group, ch;
-  int left;  // tiles of the share still to go, this segment's included
+  int b, kvh, chunk, tile, tiles, chunks, group, ch, lead;
+  int left;  // of the share, this segment included
+  int took;  // of the share, by this segment
   int seg;   // tiles of this segment
-  // tile `at` of sequence seq's work
-  __device__ __forceinline__ void start(const TreeArgs* args, int ch_, int seq, const TreeSeq& sq, unsigned long long at,
-                                        int n) {
+  // place `at` of sequence seq's work, n on from there; false: no tile among them
+  __device__ __forceinline__ bool start(const TreeArgs* args, int ch_, int lead_, int seq, const TreeSeq& sq,
+                                        unsigned long long at, int n) {
     a = args;
     ch = ch_;
+    lead = lead_;
     group = a->n_heads / a->c.n_kv;
     b = seq;
     left = n;
     s = sq;
     tiles = tree_tiles(s);
     chunks = tree_chunks(s, group, ch);
+    const int size = tiles + lead;
     unsigned long long u;
     if (at <= 0xffffffffull) {
-      u = (unsigned)at / (unsigned)tiles;
+      u = (unsigned)at / (unsigned)size;
       kvh = (int)((unsigned)u / (unsigned)chunks);
     } else {
-      u = at / tiles;
+      u = at / size;
       kvh = (int)(u / chunks);
     }
-    tile = (int)(at - u * tiles);
+    const int place = (int)(at - u * size);
     chunk = (int)(u - (unsigned long long)kvh * chunks);
-    seg = min(left, tiles - tile);
-  }
-  __device__ __forceinline__ void load() {
-    s = tree_seq(*a, b);
-    while (!s.n && b + 1 < a->n_seq) s = tree_seq(*a, ++b);
-    tiles = max(1, tree_tiles(s));
-    chunks = max(1, tree_chunks(s, group, ch));
+    took = min(left, size - place);
+    tile = max(0, place - lead);
+    seg = max(0, place + took - lead) - tile;
+    return seg > 0;
   }
   __device__ __forceinline__ bool next() {  // false: the share is done
-    left -= seg;
-    if (left <= 0) return false;
+    left -= took;
+    if (left <= lead) return false;
     tile = 0;
     if (++chunk == chunks) {
       chunk = 0;
       if (++kvh == a->c.n_kv) {
         kvh = 0;
-        b++;
-        load();
+        s = tree_seq(*a, ++b);
+        while (!s.n && b + 1 < a->n_seq) s = tree_seq(*a, ++b);
+        tiles = max(1, tree_tiles(s));
+        chunks = max(1, tree_chunks(s, group, ch));
       }
     }
-    seg = min(left, tiles);
+    took = min(left, tiles + lead);
+    seg = took - lead;
     return true;
   }
 };
@@ -350,7 +359,7 @@ struct TreeSegment {
 template <bool Q8, int NQ, int CG>
 __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_constant__ TreeTcArgs ta) {
   using S = TtShape<Q8, NQ, CG>;
-  constexpr int CH = S::CH, TG = S::TG, N = S::N, CS = S::CS;
+  constexpr int CH = S::CH, TG = S::TG, N = S::N, CS = S::CS, CO = S::CO;
   const TreeArgs& a = ta.t;
   extern __shared__ __align__(16) uint8_t smem_dyn[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~(uintptr_t)1023);
@@ -370,11 +379,14 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
   __shared__ unsigned long long col_mask[2][CH], any_mask[2];
   __shared__ int col_off[2][CH];
   __shared__ __align__(16) float col_mul[2][CH];
-  __shared__ __align__(16) float x_max[4][2][4][NQ], x_sum[4][4][NQ];
-  __shared__ __align__(16) float x_m[16][NQ], x_w[16][NQ], x_al[16][NQ], x_fold[16][2][NQ];  // per warp
+  __shared__ __align__(16) float x_max[4][4][NQ], x_sum[4][4][NQ];
+  // per warp: minus a column's reference, minus its last rise, what that does to l and o
+  __shared__ __align__(16) float x_m[16][NQ], x_d[16][NQ], x_al[16][NQ];
+  __shared__ int x_on[4];                      // does a team's O go onto what its accumulator holds?
   __shared__ float2 x_fin[4][NQ];              // (max, sum) of a finished segment
-  __shared__ unsigned long long x_bad[4][2];   // drafted rows of V that are not finite
-  __shared__ unsigned long long w_sum[TT_THREADS / 32], s_total, s_all;
+  __shared__ unsigned long long x_bad[4];   // drafted rows of V that are not finite
+  __shared__ unsigned long long w_sum[TT_THREADS / 32], s_all;
+  __shared__ int s_any;     // has the share a tile?
   __shared__ TreeWalk s_walk;  // where the share begins
   volatile int* abort = &s_abort;
 
@@ -386,6 +398,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
 
   if (tid == 0) {
     s_abort = 0;
+    s_any = 0;
     any_mask[0] = any_mask[1] = 0ull;
     for (int i = 0; i < slots; i++) {
       mbar_init(&full[0][i], 1);
@@ -405,6 +418,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
     mbar_init(&done_o, 1);
     fence_barrier_init();
   }
+  __syncthreads();
   pdl_wait();     // what comes next reads what earlier kernels wrote
   pdl_trigger();  // the merge kernel may take its place; it waits for this grid
   if (wi == TT_S_WARP) {  // after the wait: an earlier kernel may still have needed the TMEM
@@ -422,7 +436,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
       return total <= 0xffffffull ? (unsigned long long)((unsigned)total * i / shares) : total * i / shares;
     };
     auto found = [&](const TreeSeq& sq, int b, unsigned long long at, unsigned long long n) {
-      s_walk.start(&a, CH, b, sq, at, (int)n);
+      s_any = s_walk.start(&a, CH, S::LEAD, b, sq, at, (int)n);
     };
     const bool all = blockIdx.x == 0;  // CTA 0 looks for sequences that do not fit
     auto look = [&](int b, const TreeSeq& sq) {
@@ -441,35 +455,29 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
       if (wi == 0) {
         TreeSeq sq{0, 0, 0, 0};
         if (lane < n_seq) sq = tree_seq(a, lane);
-        const unsigned long long w = tree_work(sq, n_kv, group, CH), inc = scan(w);
+        const unsigned long long w = tree_work(sq, n_kv, group, CH, S::LEAD), inc = scan(w);
         const unsigned long long total = __shfl_sync(0xffffffffu, inc, 31);
         const unsigned long long t0 = share(total, blockIdx.x), t1 = share(total, blockIdx.x + 1);
-        if (lane == 0) {
-          s_total = t1 - t0;
-          s_all = total;
-        }
+        if (lane == 0) s_all = total;
         if (w && inc - w <= t0 && t0 < inc && t1 > t0) found(sq, lane, t0 - (inc - w), t1 - t0);
         if (all && lane < n_seq) look(lane, sq);
       }
     } else {
       auto seq = [&](int b) { return b < n_seq ? tree_seq(a, b) : TreeSeq{0, 0, 0, 0}; };
       unsigned long long sum = 0;
-      for (int b = tid; b < n_seq; b += TT_THREADS) sum += tree_work(seq(b), n_kv, group, CH);
+      for (int b = tid; b < n_seq; b += TT_THREADS) sum += tree_work(seq(b), n_kv, group, CH, S::LEAD);
       sum = scan(sum);
       if (lane == 31) w_sum[wi] = sum;
       __syncthreads();
       unsigned long long total = 0;
       for (int w = 0; w < TT_THREADS / 32; w++) total += w_sum[w];
       const unsigned long long t0 = share(total, blockIdx.x), t1 = share(total, blockIdx.x + 1);
-      if (tid == 0) {
-        s_total = t1 - t0;
-        s_all = total;
-      }
+      if (tid == 0) s_all = total;
       unsigned long long before = 0;
       for (int b0 = 0; b0 < n_seq && (all || (t1 > t0 && before <= t0)); b0 += TT_THREADS) {
         const int b = b0 + tid;
         const TreeSeq sq = seq(b);
-        const unsigned long long w = tree_work(sq, n_kv, group, CH), inc = scan(w);
+        const unsigned long long w = tree_work(sq, n_kv, group, CH, S::LEAD), inc = scan(w);
         __syncthreads();
         if (lane == 31) w_sum[wi] = inc;
         __syncthreads();
@@ -487,7 +495,6 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_s;
-  const int n_tiles = (int)s_total;
   // A segment's columns: q operand, masks, places.  Eight lanes a column, four
   // columns a warp at a time; this warp is number `at` of `warps`.
   auto stage = [&](const TreeSegment& sg, int set, int at, int warps) {
@@ -570,7 +577,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
   };
 
   // Team k % TG does the CTA's tile k, as its item k / TG.
-  if (n_tiles == 0) {
+  if (!s_any) {
     // nothing: fall through to the end
   } else if (wi == TT_TMA_WARP) {
     // ------------------------------------------------ TMA: K and V of every tile, slot after slot
@@ -609,12 +616,12 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
       TreeWalk w = s_walk;
       const bool scores = wi == TT_S_WARP;
       const int ks_n = Q8 ? (hd + 31) / 32 : (hd + 15) / 16;
-      constexpr uint32_t IDESC_S = tt_idesc<Q8>(N, false), IDESC_O = tt_idesc<Q8>(N, true);
+      constexpr uint32_t IDESC_S = tt_idesc<Q8>(N, false), IDESC_O = tt_idesc<Q8>(S::NO, true);
       int slot = scores ? 0 : 1, seg_left = w.seg;
       uint32_t phase = 0, segs = 0;
       int turn = 0;  // of `period` tiles, after which a slot's barrier is in its next phase
       bool fresh = true;  // a segment begins: its columns first
-      for (int k = 0; k < n_tiles && !*abort; k++) {
+      for (int k = 0; !*abort; k++) {
         const int g = k % TG;
         const uint32_t n = (uint32_t)(k / TG);
         if (scores) {
@@ -641,8 +648,6 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
           if (fresh) {
             tc_commit(&q_free);
             segs++;
-            if (k + 1 < n_tiles) w.next();
-            seg_left = w.seg;
           }
         } else {
           tt_wait(&p_full[g], n & 1, abort);
@@ -653,15 +658,18 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
           // halves (the upper half of O is not read)
           const uint64_t vd = sw128_desc_mn(smem_u32(base + slot * slot_bytes), boxes == 2 ? 16384u : 0u, 1024u);
           const uint64_t pd = sw64_desc_mn(smem_u32(base + S::OFF_P + g * S::PSZ));
+          const uint32_t d = tmem + TG * CS + g * CO;
+          const bool on = x_on[g] != 0;      // onto the tiles before this one
           constexpr int STEPS = Q8 ? 4 : 8;  // 32 or 16 positions each
 #pragma unroll
           for (int ks = 0; ks < STEPS; ks++) {
             if constexpr (Q8)
-              tc_mma_i8_acc(tmem + (TG + g) * CS, vd + ks * 256, pd + ks * 128, IDESC_O, ks > 0);
+              tc_mma_i8_acc(d, vd + ks * 256, pd + ks * 128, IDESC_O, ks > 0 || on);
             else
-              tc_mma_f16(tmem + (TG + g) * CS, vd + ks * 128, pd + ks * 64, IDESC_O, ks > 0);
+              tc_mma_f16(d, vd + ks * 128, pd + ks * 64, IDESC_O, ks > 0 || on);
           }
           tc_commit(&o_full[g]);
+          fresh = --seg_left == 0;
         }
         tc_commit(&empty[slot]);
         slot += 2;  // K and V alternate
@@ -669,6 +677,10 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
         if (++turn == period) {
           turn = 0;
           phase ^= 1;
+        }
+        if (fresh) {
+          if (!w.next()) break;
+          seg_left = w.seg;
         }
       }
       // wind down: every MMA issued has completed before TMEM is freed
@@ -709,7 +721,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
     const int g = wi >> 2, wq = wi & 3, r = tid & 127, tg = g / CG, cg = g % CG;
     const uint32_t lanes = (uint32_t)(wq * 32) << 16;
     const int c0 = cg * NQ;  // of the team's columns
-    const uint32_t s_at = tmem + lanes + (uint32_t)(tg * CS + c0), o_at = tmem + lanes + (uint32_t)((TG + tg) * CS + c0);
+    const uint32_t s_at = tmem + lanes + (uint32_t)(tg * CS + c0), o_at = tmem + lanes + (uint32_t)(TG * CS + tg * CO + c0);
     uint8_t* p_t = base + S::OFF_P + tg * S::PSZ;
     const bool has_dim = wq * 32 < hd;  // this warp's lanes of O are dims
     int item = 0;  // of this group, over all segments
@@ -729,6 +741,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
       const TreeSegment& sg = seg_tab[set];
       const int len = sg.len, total = sg.total, tiles = sg.tiles;
       const int first = (tg - k0) & (TG - 1);
+      const bool trees = total - len > 1;
       const float *ks_at = nullptr, *vs_at = nullptr;
       float ks_next = 0.0f, vs_next = 0.0f;
       auto scales = [&](int t) {  // of tile t's place r, and on to the group's next tile
@@ -745,76 +758,64 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
         scales(first);
       }
       F2 l[NQ / 2], o[NQ / 2];
-      float R = -INFINITY;  // lane c holds the running maximum of column c
+      float ref = -INFINITY;  // lane c: the reference of column c; none yet
+      int run = 0;            // tiles against the present references
+      bool held = false;      // O holds tiles that are not in o
 #pragma unroll
       for (int c = 0; c < NQ / 2; c++) l[c] = o[c] = F2(0.0f);
+      if (!Q8 && r == 0) x_bad[g] = 0ull;
 
-      // O of the group's previous item into the registers
-      auto fold = [&](int par) {
+      // O into the registers
+      auto fold = [&]() {
         tt_wait(&o_full[tg], (uint32_t)(item - 1) & 1, abort);
         tc_fence_after();
         if (has_dim) {
+          const F2 unit(1.0f / TT_UNITS<Q8>);
 #pragma unroll
           for (int cb = 0; cb < NQ; cb += 8) {
-            uint32_t v[24];
-            tt_ld<8>(o_at + cb, v);
-            tt_ld<8>(o_at + CH + cb, v + 8);
-            if constexpr (Q8) tt_ld<8>(o_at + 2 * CH + cb, v + 16);
+            uint32_t v[32];
+            tc_ld8(o_at + cb, v);
+            tc_ld8(o_at + CH + cb, v + 8);
+            if constexpr (Q8) {
+              tc_ld8(o_at + 2 * CH + cb, v + 16);
+              tc_ld8(o_at + 3 * CH + cb, v + 24);
+            }
             tc_wait_ld();
 #pragma unroll
-            for (int c = 0; c < 8; c += 4) {
-              const float4 f = *reinterpret_cast<const float4*>(&x_fold[wi][par][cb + c]);
-              F2& o0 = o[(cb + c) / 2];
-              F2& o1 = o[(cb + c) / 2 + 1];
-              o0 = fma2(joined<Q8, 8>(v, c), F2(f.x, f.y), o0);
-              o1 = fma2(joined<Q8, 8>(v, c + 2), F2(f.z, f.w), o1);
+            for (int c = 0; c < 8; c += 2) {
+              F2& x = o[(cb + c) / 2];
+              if constexpr (Q8) {
+                const F2 k(256.0f);
+                auto digit = [&](int z) { return F2((float)(int)v[8 * z + c], (float)(int)v[8 * z + c + 1]); };
+                x = fma2(fma2(fma2(fma2(digit(0), k, digit(1)), k, digit(2)), k, digit(3)), unit, x);
+              } else {
+                x = fma2(joined<false, 8>(v, c), unit, x);
+              }
             }
           }
         }
         tc_fence_before();
-        if constexpr (!Q8) {  // drafted rows of V that are not finite: nodes that see them get NaN
-          unsigned long long bad = x_bad[g][par];
-          while (bad) {
-            const int j = __ffsll((long long)bad) - 1;
-            bad &= bad - 1;
-            float v = 0.0f;
-            if (r < hd)
-              v = __half2float(static_cast<const __half*>(a.c.v)[(size_t)(sg.row + len + j) * a.c.row_stride +
-                                                                (size_t)sg.kvh * a.c.head_stride + r]);
-            if (!(fabsf(v) < INFINITY)) {
-              const float nan = __int_as_float(0x7fffffff);
-#pragma unroll
-              for (int c = 0; c < NQ; c += 2)
-                o[c / 2] = F2(col_mask[set][c0 + c] >> j & 1 ? nan : o[c / 2].lo(),
-                              col_mask[set][c0 + c + 1] >> j & 1 ? nan : o[c / 2].hi());
-            }
-          }
-        }
       };
 
-      int done = 0;  // items of this segment
-      for (int t = first; t < tiles; t += TG, item++, done++) {
-        const int par = item & 1, pos = t * TT_TILE + r, j = pos - len;
+      for (int t = first; t < tiles; t += TG, item++) {
+        const int pos = t * TT_TILE + r, j = pos - len;
         const bool edge = (t + 1) * TT_TILE > len;  // drafted places or none at all among the tile's
         const bool there = pos < total;
         // an f16 edge tile: which 8-value pieces of this drafted V row are not finite
         uint32_t odd = 0;
         if constexpr (!Q8) {
-          if (edge) {
-            if (r == 0) x_bad[g][par] = 0ull;
-            if (there && j >= 0 && (any_mask[set] >> j & 1)) {
-              const uint4* v = reinterpret_cast<const uint4*>(static_cast<const __half*>(a.c.v) +
-                                                              (size_t)(sg.row + pos) * a.c.row_stride +
-                                                              (size_t)sg.kvh * a.c.head_stride);
-              for (int c = 0; c < hd / 8; c++) {
-                const uint4 x = v[c];
-                const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
-                bool bad = false;
+          if (edge && there && j >= 0 && (any_mask[set] >> j & 1)) {
+            const uint4* v = reinterpret_cast<const uint4*>(static_cast<const __half*>(a.c.v) +
+                                                            (size_t)(sg.row + pos) * a.c.row_stride +
+                                                            (size_t)sg.kvh * a.c.head_stride);
+            for (int c = 0; c < hd / 8; c++) {
+              const uint4 x = v[c];
+              const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+              bool bad = false;
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                  bad |= (xs[e] & 0x7c00u) == 0x7c00u || (xs[e] & 0x7c000000u) == 0x7c000000u;
-                odd |= (uint32_t)bad << c;
-              }
+              for (int e = 0; e < 4; e++)
+                bad |= (xs[e] & 0x7c00u) == 0x7c00u || (xs[e] & 0x7c000000u) == 0x7c000000u;
+              odd |= (uint32_t)bad << c;
             }
           }
         }
@@ -835,7 +836,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
             vm = __uint_as_float((b & 0x007fffffu) | 0x3f800000u);
           }
         }
-        // ---- scores (with V's exponent), in powers of two
+        // ---- scores (with V's exponent), in powers of two, against the references
         tt_wait(&s_full[tg], (uint32_t)item & 1, abort);
         tc_fence_after();
         constexpr int W = NQ;  // columns of one load: each wait for TMEM costs its whole latency
@@ -872,89 +873,104 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
             s[c / 2] = F2(s0 ? s[c / 2].lo() : -INFINITY, s1 ? s[c / 2].hi() : -INFINITY);
           }
         }
-        // ---- the tile's maximum of every column
+        // tiles with drafted places set the references anew each: whether another
+        // node's score passes its reference must not touch this one's sums
+        bool fresh = run == 0 || run == TT_RUN || (edge && trees);
+        if (run) {
+          float top = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < NQ; c += 4) {
-          float4 m;
-          m.x = redux_max(s[c / 2].lo());
-          m.y = redux_max(s[c / 2].hi());
-          m.z = redux_max(s[c / 2 + 1].lo());
-          m.w = redux_max(s[c / 2 + 1].hi());
-          if (lane == 0) *reinterpret_cast<float4*>(&x_max[g][par][wq][c]) = m;
-        }
-        group_sync(g);
-        float al = 1.0f;
-        if (lane < NQ) {
-          const float m = fmaxf(fmaxf(x_max[g][par][0][lane], x_max[g][par][1][lane]),
-                                fmaxf(x_max[g][par][2][lane], x_max[g][par][3][lane]));
-          const float top = fmaxf(R, m);
-          const float wt = m == -INFINITY ? 0.0f : ex2(m - top);
-          if (R != -INFINITY) al = ex2(R - top);
-          R = top;
-          x_m[wi][lane] = m == -INFINITY ? 0.0f : -m;
-          x_w[wi][lane] = wt;
-          x_al[wi][lane] = al;
-          x_fold[wi][par][lane] = wt * (Q8 ? 2.0f / TT_DIGITS : 0x1p-15f);
-        }
-        const bool moved = __any_sync(0xffffffffu, al != 1.0f);
-        if (done) fold(par ^ 1);
-        __syncwarp();
-        if (moved) {
-#pragma unroll
-          for (int c = 0; c < NQ; c += 2) {
-            const F2 f(x_al[wi][c], x_al[wi][c + 1]);
-            l[c / 2] = l[c / 2] * f;
-            o[c / 2] = o[c / 2] * f;
+          for (int c = 0; c < NQ; c += 4) {
+            const float4 m = *reinterpret_cast<const float4*>(&x_m[wi][c]);
+            s[c / 2] = s[c / 2] + F2(m.x, m.y);
+            s[c / 2 + 1] = s[c / 2 + 1] + F2(m.z, m.w);
+            top = fmaxf(fmaxf(top, fmaxf(s[c / 2].lo(), s[c / 2].hi())), fmaxf(s[c / 2 + 1].lo(), s[c / 2 + 1].hi()));
           }
+          if (!fresh) fresh = team_any<CG>(tg, top > TT_ROOM);
+        }
+        if (fresh) {
+          // ---- what O holds, then the references: a column's largest score so far
+#pragma unroll
+          for (int c = 0; c < NQ; c += 4) {
+            float4 m;
+            m.x = redux_max(s[c / 2].lo());
+            m.y = redux_max(s[c / 2].hi());
+            m.z = redux_max(s[c / 2 + 1].lo());
+            m.w = redux_max(s[c / 2 + 1].hi());
+            if (lane == 0) *reinterpret_cast<float4*>(&x_max[g][wq][c]) = m;
+          }
+          group_sync(g);
+          if (held) fold();
+          held = false;
+          if (lane < NQ) {
+            // against the old reference, or against 0 where there is none
+            const float m = fmaxf(fmaxf(x_max[g][0][lane], x_max[g][1][lane]), fmaxf(x_max[g][2][lane], x_max[g][3][lane]));
+            const bool none = ref == -INFINITY;
+            const float up = none ? (m == -INFINITY ? 0.0f : m) : fmaxf(m, 0.0f);
+            x_al[wi][lane] = none ? 1.0f : ex2(-up);
+            if (!none) ref += up;
+            else if (m != -INFINITY) ref = m;
+            x_m[wi][lane] = ref == -INFINITY ? 0.0f : -ref;
+            x_d[wi][lane] = -up;
+          }
+          group_sync(g);  // the tables are written, and x_max may be again
+#pragma unroll
+          for (int c = 0; c < NQ; c += 4) {
+            const float4 m = *reinterpret_cast<const float4*>(&x_d[wi][c]), al = *reinterpret_cast<const float4*>(&x_al[wi][c]);
+            s[c / 2] = s[c / 2] + F2(m.x, m.y);
+            s[c / 2 + 1] = s[c / 2 + 1] + F2(m.z, m.w);
+            l[c / 2] = l[c / 2] * F2(al.x, al.y);
+            l[c / 2 + 1] = l[c / 2 + 1] * F2(al.z, al.w);
+            o[c / 2] = o[c / 2] * F2(al.x, al.y);
+            o[c / 2 + 1] = o[c / 2 + 1] * F2(al.z, al.w);
+          }
+          run = 0;
         }
         // ---- probabilities, in the operand's form, a row per position
         if constexpr (Q8) {
           const bool tiny = ve < -60;  // such a place's weight may be lost beside p * 2^ve: it is summed by itself
           if (__any_sync(0xffffffffu, tiny)) {
 #pragma unroll
-            for (int c = 0; c < NQ; c += 2) {
-              const float p0 = tiny ? ex2((s[c / 2].lo() + x_m[wi][c]) - (float)ve) : 0.0f;
-              const float p1 = tiny ? ex2((s[c / 2].hi() + x_m[wi][c + 1]) - (float)ve) : 0.0f;
-              l[c / 2] = fma2(F2(p0, p1), F2(x_w[wi][c], x_w[wi][c + 1]), l[c / 2]);
-            }
+            for (int c = 0; c < NQ; c += 2)
+              if (tiny) l[c / 2] = l[c / 2] + F2(ex2(s[c / 2].lo() - (float)ve), ex2(s[c / 2].hi() - (float)ve));
           }
-          const F2 cm(vm * (0.5f * TT_DIGITS)), iv(tiny ? 0.0f : __uint_as_float((uint32_t)(127 - ve) << 23)), bias(TT_BIAS);
-          uint32_t dg[3][NQ / 4];
+          const F2 cm(vm * TT_UNITS<true>), iv(tiny ? 0.0f : __uint_as_float((uint32_t)(127 - ve) << 23));
+          uint32_t dg[4][NQ / 4];
 #pragma unroll
           for (int c = 0; c < NQ; c += 4) {
-            const float4 m = *reinterpret_cast<const float4*>(&x_m[wi][c]);
-            const float4 wt = *reinterpret_cast<const float4*>(&x_w[wi][c]);
-            const F2 d0 = s[c / 2] + F2(m.x, m.y), d1 = s[c / 2 + 1] + F2(m.z, m.w);
-            const F2 p0(ex2(d0.lo()), ex2(d0.hi())), p1(ex2(d1.lo()), ex2(d1.hi()));
-            l[c / 2] = fma2(p0 * iv, F2(wt.x, wt.y), l[c / 2]);
-            l[c / 2 + 1] = fma2(p1 * iv, F2(wt.z, wt.w), l[c / 2 + 1]);
-            const F2 f0 = fma2(p0, cm, bias), f1 = fma2(p1, cm, bias);
-            const uint32_t f[4] = {__float_as_uint(f0.lo()), __float_as_uint(f0.hi()), __float_as_uint(f1.lo()),
-                                   __float_as_uint(f1.hi())};
+            const F2 p0(ex2(s[c / 2].lo()), ex2(s[c / 2].hi())), p1(ex2(s[c / 2 + 1].lo()), ex2(s[c / 2 + 1].hi()));
+            l[c / 2] = fma2(p0, iv, l[c / 2]);
+            l[c / 2 + 1] = fma2(p1, iv, l[c / 2 + 1]);
+            const F2 f0 = p0 * cm, f1 = p1 * cm;
+            // balanced digits: bytes of the value + 0x808080, the lower three less 128
+            const uint32_t f[4] = {(uint32_t)__float2int_rn(f0.lo()) + 0x808080u, (uint32_t)__float2int_rn(f0.hi()) + 0x808080u,
+                                   (uint32_t)__float2int_rn(f1.lo()) + 0x808080u, (uint32_t)__float2int_rn(f1.hi()) + 0x808080u};
             const uint32_t a01 = __byte_perm(f[0], f[1], 0x5140), a23 = __byte_perm(f[2], f[3], 0x5140);
-            dg[2][c / 4] = __byte_perm(a01, a23, 0x5410) ^ 0x80808080u;
-            dg[1][c / 4] = __byte_perm(a01, a23, 0x7632) ^ 0x80808080u;
-            dg[0][c / 4] = __byte_perm(__byte_perm(f[0], f[1], 0x0062), __byte_perm(f[2], f[3], 0x0062), 0x5410);
+            const uint32_t b01 = __byte_perm(f[0], f[1], 0x7362), b23 = __byte_perm(f[2], f[3], 0x7362);
+            dg[3][c / 4] = __byte_perm(a01, a23, 0x5410) ^ 0x80808080u;
+            dg[2][c / 4] = __byte_perm(a01, a23, 0x7632) ^ 0x80808080u;
+            dg[1][c / 4] = __byte_perm(b01, b23, 0x5410) ^ 0x80808080u;
+            dg[0][c / 4] = __byte_perm(b01, b23, 0x7632);
           }
+          if (item) tt_wait(&o_full[tg], (uint32_t)(item - 1) & 1, abort);  // the p operand has been read
           if constexpr (NQ == 16) {
 #pragma unroll
-            for (int z = 0; z < 3; z++)
+            for (int z = 0; z < 4; z++)
               *reinterpret_cast<uint4*>(p_t + sw64(r, z * CG + cg)) = make_uint4(dg[z][0], dg[z][1], dg[z][2], dg[z][3]);
           } else {
             *reinterpret_cast<uint4*>(p_t + sw64(r, 0)) = make_uint4(dg[0][0], dg[0][1], dg[1][0], dg[1][1]);
-            *reinterpret_cast<uint4*>(p_t + sw64(r, 1)) = make_uint4(dg[2][0], dg[2][1], 0u, 0u);
+            *reinterpret_cast<uint4*>(p_t + sw64(r, 1)) = make_uint4(dg[2][0], dg[2][1], dg[3][0], dg[3][1]);
           }
         } else {
+          if (item) tt_wait(&o_full[tg], (uint32_t)(item - 1) & 1, abort);  // the p operand has been read
 #pragma unroll
           for (int cb = 0; cb < NQ; cb += 8) {
             uint32_t hi[4], lo[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
               const int c = cb + e * 2;
-              const F2 d = s[c / 2] + F2(x_m[wi][c], x_m[wi][c + 1]);
-              const F2 p(ex2(d.lo()), ex2(d.hi()));
-              l[c / 2] = fma2(p, F2(x_w[wi][c], x_w[wi][c + 1]), l[c / 2]);
-              const F2 x = p * F2(32768.0f);  // far from f16's smallest values
+              const F2 p(ex2(s[c / 2].lo()), ex2(s[c / 2].hi()));
+              l[c / 2] = l[c / 2] + p;
+              const F2 x = p * F2(TT_UNITS<false>);  // far from f16's smallest values
               const F2 h(__uint_as_float(__float_as_uint(x.lo()) & 0xffffe000u), __uint_as_float(__float_as_uint(x.hi()) & 0xffffe000u));
               const F2 rest = fma2(h, F2(-1.0f), x);
               const __half2 hh = __floats2half2_rn(h.lo(), h.hi()), dd = __floats2half2_rn(rest.lo(), rest.hi());
@@ -987,17 +1003,36 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
                     *at = x;
                   }
                 }
-              if (odd) atomicOr(&x_bad[g][par], 1ull << j);
+              if (odd) atomicOr(&x_bad[g], 1ull << j);
             }
-          } else if (r == 0) {
-            x_bad[g][par] = 0ull;
           }
         }
+        if (r == 0 && cg == 0) x_on[tg] = held;
+        held = true;
+        run++;
         fence_async_smem();
         mbar_arrive(&p_full[tg]);
-        if constexpr (!Q8) group_sync(g);  // x_bad is whole before the fold reads it
       }
-      if (done) fold((item - 1) & 1);
+      if (held) fold();
+      if constexpr (!Q8) {  // drafted rows of V that are not finite: nodes that see them get NaN
+        group_sync(g);
+        unsigned long long bad = x_bad[g];
+        while (bad) {
+          const int j = __ffsll((long long)bad) - 1;
+          bad &= bad - 1;
+          float v = 0.0f;
+          if (r < hd)
+            v = __half2float(static_cast<const __half*>(a.c.v)[(size_t)(sg.row + len + j) * a.c.row_stride +
+                                                              (size_t)sg.kvh * a.c.head_stride + r]);
+          if (!(fabsf(v) < INFINITY)) {
+            const float nan = __int_as_float(0x7fffffff);
+#pragma unroll
+            for (int c = 0; c < NQ; c += 2)
+              o[c / 2] = F2(col_mask[set][c0 + c] >> j & 1 ? nan : o[c / 2].lo(),
+                            col_mask[set][c0 + c + 1] >> j & 1 ? nan : o[c / 2].hi());
+          }
+        }
+      }
 
       // ---- the segment's (max, sum, o): the groups of a column range meet through their idle p operands
 #pragma unroll
@@ -1013,7 +1048,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
       }
       group_sync(g);
       if (wq == 0 && lane < NQ)
-        x_fin[g][lane] = make_float2(R, (x_sum[g][0][lane] + x_sum[g][1][lane]) + (x_sum[g][2][lane] + x_sum[g][3][lane]));
+        x_fin[g][lane] = make_float2(ref, (x_sum[g][0][lane] + x_sum[g][1][lane]) + (x_sum[g][2][lane] + x_sum[g][3][lane]));
       groups_sync();
       {
         const bool whole = sg.first && !sg.rest;
