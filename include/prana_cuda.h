@@ -245,9 +245,10 @@ int prana_kv_rows_move(prana_ctx *ctx, const prana_kv_rows *cache, const int32_t
  * row NaN.
  * workspace: NULL for the context's scratch (then calls on several streams must
  * not overlap), or workspace_bytes of 256-byte aligned device memory, at least
- * what prana_attention_tree_workspace says, not shared by overlapping calls;
- * its contents do not matter.  With a workspace the call allocates nothing and
- * can be captured into a graph. */
+ * what prana_attention_tree_workspace says, not shared by overlapping calls.
+ * Zero its first 4096 bytes before its first use (and after PRANA_E_TIMEOUT):
+ * every call finds counters there at zero and leaves them so.  With a workspace
+ * the call allocates nothing and can be captured into a graph. */
 int prana_attention_tree_workspace(prana_ctx *ctx, size_t max_nodes, size_t n_heads, size_t n_kv_heads, size_t head_dim,
                                    size_t *bytes);
 int prana_attention_tree(prana_ctx *ctx, const float *q, const prana_kv_rows *cache, const int32_t *starts,

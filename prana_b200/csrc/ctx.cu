@@ -247,6 +247,8 @@ int prana_ctx_synchronize(prana_ctx* c) {
   PRANA_CK(cudaMemcpy(&e, c->err, sizeof(unsigned), cudaMemcpyDeviceToHost));
   if (e) PRANA_CK(cudaMemset(c->err, 0, sizeof(unsigned)));
   if (int rc = noalloc_take_error(c->device, &e2)) return rc;
+  // a kernel that gave up may not have drawn all of its tickets
+  if (e & ERR_TIMEOUT) PRANA_CK(cudaMemset(c->counters, 0, 4096 * sizeof(unsigned)));
   if ((e & ERR_TIMEOUT) || e2)
     return fail(PRANA_E_TIMEOUT, "a bounded device-side wait expired in a kernel-level call (%s)",
                 e ? "context" : "no-allocation attention");
@@ -705,8 +707,9 @@ int prana_attention_tree(prana_ctx* c, const float* q, const prana_kv_rows* cach
     NEED(workspace_bytes >= need, "the workspace has %zu bytes; %zu are needed", workspace_bytes, need);
     NEED(aligned_to(workspace, 256), "the workspace must be 256-byte aligned");
     a.work = workspace;
-  } else if (int rc = ctx_scratch(c, need, &a.work)) {
-    return rc;
+  } else {
+    if (int rc = ctx_scratch(c, need, &a.work)) return rc;
+    a.tickets = c->counters;
   }
   a.q = q;
   a.starts = starts;

@@ -227,6 +227,7 @@ struct TreeArgs {
   int n_seq, n_nodes, max_nodes, n_heads;
   float* out;  // [n_nodes][n_heads * hd]
   void* work;
+  unsigned* tickets;  // null: at the start of work
   unsigned* err;
   int sm_count, device;
 };

@@ -148,8 +148,8 @@ constexpr float TT_UNITS = Q8 ? 2139000000.0f / 512.0f : 128.0f;
 constexpr int TT_RUN = 512;
 constexpr float LOG2E = 1.4426950408889634f;
 
-// What a CTA leaves for the merge: the unit that began in it and went on in
-// the next n - 1 CTAs (n = 0: none).
+// What a CTA leaves for tree_merge_kernel: the unit that began in it and went on
+// in the next n - 1 CTAs (n = 0: none).
 struct TreePart {
   int n, cols, vh0, kvh, off, pad[3];
 };
@@ -158,6 +158,7 @@ struct TreeTcArgs {
   TreeArgs t;
   int boxes;        // TMA boxes of a tile's K (or V): 1, or 2 for an f16 head above 64
   int slots;        // ring slots
+  unsigned* tickets;  // [CTAs], zero between calls: the shares of the unit that began in a CTA that are done
   TreePart* parts;  // [CTAs]
   float2* part_ml;  // [2 * CTAs][columns] (max, sum)
   float* part_o;    // [2 * CTAs][columns][hd]
@@ -177,6 +178,10 @@ struct TtShape {
   static constexpr int RING = (CG < 4 ? 160 : 128) * 1024;
   static constexpr int OFF_P = RING, OFF_Q = OFF_P + TG * PSZ;
   static constexpr size_t BYTES = 1024 + OFF_Q + QSZ;
+  // Who adds a unit's partials up: the CTA that is done last, which saves a launch
+  // and its two waits (4 us of a call); 64 columns are more than one SM reads in
+  // that time (600 KB of a 4096 context), and a kernel follows.
+  static constexpr bool TICKET = CH <= 32;
   static_assert(TG * (CS + CO) <= 512, "TMEM");
   // a segment's start and end, in tiles (8 to 14 thousand cycles against 1.5 of a decode tile, 4 of a wide one)
   static constexpr int LEAD = CG == 1 ? 4 : 2;
@@ -345,16 +350,59 @@ struct TreeWalk {
     seg = took - lead;
     return true;
   }
+  __device__ __forceinline__ bool more() const { return left - took > lead; }
 };
 
 // What the softmax groups need of a segment; places count from its first tile.
 struct TreeSegment {
   int row, len, total, off;  // cache row of place 0; places all nodes see; places; first query row
   int kvh, tiles;
-  int first, rest;           // does the unit begin here; its tiles after this segment
+  int before, rest;          // the unit's tiles before and after this segment
   int vh0, cols;             // the chunk's first column of the unit, and its columns
   int more;                  // another segment follows
 };
+
+// Column c of a unit whose n partials lie in the CTAs from i0: every STEP-th from
+// `from` on, weighed by the maximum of all, onto x (the dims lane + 32 e); returns
+// the sum of all.  The order is that of the tiles, whoever does it.
+template <int STEP>
+__device__ __forceinline__ float tree_add(const TreeTcArgs& ta, int ch, int c, int i0, int n, int from, int lane, int hd,
+                                          float (&x)[4]) {
+  auto slot = [&](int i) { return (2 * (size_t)(i0 + i) + (i == 0 ? 1 : 0)) * ch + c; };
+  float m = -INFINITY, sum = 0.0f;
+  for (int i = lane; i < n; i += 32) m = fmaxf(m, __ldcg(&ta.part_ml[slot(i)]).x);
+  m = warp_max(m);
+  for (int ib = 0; ib < n; ib += 32) {
+    float wt = 0.0f;
+    if (ib + lane < n) {
+      const float2 f = __ldcg(&ta.part_ml[slot(ib + lane)]);
+      wt = f.x == -INFINITY ? 0.0f : ex2(f.x - m);
+      sum = fmaf(f.y, wt, sum);
+    }
+#pragma unroll 8
+    for (int i = from; i < min(32, n - ib); i += STEP) {
+      const float f = __shfl_sync(0xffffffffu, wt, i);
+      const float* po = ta.part_o + slot(ib + i) * hd;
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (e * 32 + lane < hd) x[e] = fmaf(__ldcg(po + e * 32 + lane), f, x[e]);
+    }
+  }
+  return warp_sum(sum);
+}
+// A ticket of a count over CTAs: what this CTA wrote (the others' writes ordered
+// before by the caller's barrier) is released, and the last to draw acquires it all.
+__device__ __forceinline__ unsigned ticket_acq_rel(unsigned* counter) {
+  unsigned old;
+  asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(old) : "l"(counter) : "memory");
+  return old;
+}
+
+__device__ __forceinline__ TreeSegment tree_segment(const TreeWalk& w) {
+  const int skip = w.tile * TT_TILE, vh0 = w.chunk * w.ch;
+  return TreeSegment{w.s.start + skip, w.s.len - skip, w.s.len + w.s.n - skip, w.s.off, w.kvh, w.seg, w.tile,
+                     w.tiles - w.tile - w.seg, vh0, min(w.ch, w.s.n * w.group - vh0), w.more()};
+}
 
 template <bool Q8, int NQ, int CG>
 __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_constant__ TreeTcArgs ta) {
@@ -386,7 +434,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
   __shared__ float2 x_fin[4][NQ];              // (max, sum) of a finished segment
   __shared__ unsigned long long x_bad[4];   // drafted rows of V that are not finite
   __shared__ unsigned long long w_sum[TT_THREADS / 32], s_all;
-  __shared__ int s_any;     // has the share a tile?
+  __shared__ int s_any;       // has the share a tile?
+  __shared__ int s_merge[2];  // partials for this CTA to add up (0: not its turn), the first's CTA
   __shared__ TreeWalk s_walk;  // where the share begins
   volatile int* abort = &s_abort;
 
@@ -437,6 +486,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
     };
     auto found = [&](const TreeSeq& sq, int b, unsigned long long at, unsigned long long n) {
       s_any = s_walk.start(&a, CH, S::LEAD, b, sq, at, (int)n);
+      seg_tab[0] = tree_segment(s_walk);
     };
     const bool all = blockIdx.x == 0;  // CTA 0 looks for sequences that do not fit
     auto look = [&](int b, const TreeSeq& sq) {
@@ -450,7 +500,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
       }
       return x;
     };
-    if (tid == 0) ta.parts[blockIdx.x].n = 0;
+    if (!S::TICKET && tid == 0) ta.parts[blockIdx.x].n = 0;
     if (n_seq <= 32) {  // one warp sees them all
       if (wi == 0) {
         TreeSeq sq{0, 0, 0, 0};
@@ -691,31 +741,21 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
     __syncwarp();
   } else if (wi == TT_Q_WARP) {
     // ------------------------------------------------ the next segment's columns: q operand, masks, places
+    stage(seg_tab[0], 0, TT_SOFT / 32, TT_SOFT / 32 + 1);
+    first_sync();
+    mbar_arrive(&q_ready);
     TreeWalk w = s_walk;
-    int seg = 0;
-    bool more;
-    do {
-      const int set = seg & 1, cols = min(CH, w.s.n * group - w.chunk * CH);
+    for (int seg = 1; w.next(); seg++) {
+      const int set = seg & 1;
       // everybody is in the last segment, so the set's readers, two segments ago, are done
-      if (seg) tt_wait(&q_seen, (uint32_t)(seg - 1) & 1, abort);
+      tt_wait(&q_seen, (uint32_t)(seg - 1) & 1, abort);
+      tt_wait(&q_free, (uint32_t)(seg - 1) & 1, abort);  // the last segment's products have read the operand
       if (*abort) break;
-      TreeSegment sg{w.s.start + w.tile * TT_TILE, w.s.len - w.tile * TT_TILE, w.s.len + w.s.n - w.tile * TT_TILE, w.s.off,
-                     w.kvh, w.seg, w.tile == 0, w.tiles - w.tile - w.seg, w.chunk * CH, cols, 0};
-      if (seg) {
-        tt_wait(&q_free, (uint32_t)(seg - 1) & 1, abort);  // the last segment's products have read the operand
-        stage(sg, set, 0, 1);
-      } else {
-        if (lane == 0) seg_tab[0] = sg;
-        first_sync();
-        stage(sg, 0, TT_SOFT / 32, TT_SOFT / 32 + 1);
-        first_sync();
-      }
-      more = w.next();
-      sg.more = more;
+      const TreeSegment sg = tree_segment(w);
       if (lane == 0) seg_tab[set] = sg;
+      stage(sg, set, 0, 1);
       mbar_arrive(&q_ready);
-      seg++;
-    } while (more && !*abort);
+    }
   } else {
     // ------------------------------------------------ softmax groups
     const int g = wi >> 2, wq = wi & 3, r = tid & 127, tg = g / CG, cg = g % CG;
@@ -727,16 +767,14 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
     int item = 0;  // of this group, over all segments
     int k0 = 0;    // tiles of the CTA before this segment
     int seg_no = 0, more;
-    // the first segment's columns are everybody's work
-    first_sync();
-    stage(seg_tab[0], 0, wi, TT_SOFT / 32 + 1);
-    first_sync();
     do {
       const int set = seg_no & 1;
-      tt_wait(&q_ready, (uint32_t)seg_no & 1, abort);  // the segment and its columns' tables
-      // one decision for all, so that the named barriers stay matched; from here
-      // on the last segment's p operands are free
-      if (groups_any(*abort != 0)) break;
+      if (seg_no) {
+        tt_wait(&q_ready, (uint32_t)seg_no & 1, abort);  // the segment and its columns' tables
+        // one decision for all, so that the named barriers stay matched; from here
+        // on the last segment's p operands are free
+        if (groups_any(*abort != 0)) break;
+      }
       if (tid == 0) mbar_arrive(&q_seen);
       const TreeSegment& sg = seg_tab[set];
       const int len = sg.len, total = sg.total, tiles = sg.tiles;
@@ -756,6 +794,10 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
         ks_at = a.c.k_scale + at;
         vs_at = a.c.v_scale + at;
         scales(first);
+      }
+      if (seg_no == 0) {  // the first segment's columns are everybody's work
+        stage(sg, 0, wi, TT_SOFT / 32 + 1);
+        first_sync();
       }
       F2 l[NQ / 2], o[NQ / 2];
       float ref = -INFINITY;  // lane c: the reference of column c; none yet
@@ -1051,8 +1093,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
         x_fin[g][lane] = make_float2(ref, (x_sum[g][0][lane] + x_sum[g][1][lane]) + (x_sum[g][2][lane] + x_sum[g][3][lane]));
       groups_sync();
       {
-        const bool whole = sg.first && !sg.rest;
-        const size_t slot = 2 * (size_t)blockIdx.x + (sg.first ? 1 : 0);
+        const bool first_part = sg.before == 0, whole = first_part && !sg.rest;
+        const size_t slot = 2 * (size_t)blockIdx.x + (first_part ? 1 : 0);
         const int cols = sg.cols;
         float* out_seq = a.out + (size_t)sg.off * a.n_heads * hd;
         auto put = [&](int c, float m, float sum, float x) {  // column c: final, or a partial
@@ -1082,16 +1124,56 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
             put(c, m, sum, x);
           }
         }
-        if (tid == 0 && sg.first && !whole) {  // the unit goes on in the next CTAs
-          const unsigned long long shares = s_all < gridDim.x ? s_all : gridDim.x;
-          const unsigned long long t1 = s_all * (blockIdx.x + 1) / shares;  // the end of this share
-          const unsigned long long u1 = t1 + (unsigned long long)sg.rest;
-          TreePart* pt = ta.parts + blockIdx.x;
-          pt->cols = cols;
-          pt->vh0 = sg.vh0;
-          pt->kvh = sg.kvh;
-          pt->off = sg.off;
-          pt->n = (int)((u1 * shares - 1) / s_all) - (int)blockIdx.x + 1;
+        if (!whole) {
+          if (S::TICKET) {
+            __threadfence();
+            groups_sync();
+          }
+          if (tid == 0) {
+            // the unit's tiles among all places, and the CTAs they went to
+            const unsigned long long shares = s_all < gridDim.x ? s_all : gridDim.x;
+            const int all = sg.before + tiles + sg.rest;
+            const unsigned long long u0 = first_part ? s_all * (blockIdx.x + 1) / shares - tiles : s_all * blockIdx.x / shares - sg.before;
+            const int i0 = (int)(((u0 + 1) * shares - 1) / s_all), n = (int)(((u0 + all) * shares - 1) / s_all) - i0 + 1;
+            if constexpr (S::TICKET) {
+              const bool last = ticket_acq_rel(ta.tickets + i0) == (unsigned)n - 1;
+              if (last) ta.tickets[i0] = 0u;
+              s_merge[0] = last ? n : 0;
+              s_merge[1] = i0;
+            } else if (first_part) {
+              ta.parts[blockIdx.x] = TreePart{n, cols, sg.vh0, sg.kvh, sg.off, {0, 0, 0}};
+            }
+          }
+          if constexpr (S::TICKET) {
+            groups_sync();
+            if (s_merge[0]) {
+              // the last of them: one warp a column (or two, with half the partials each)
+              const int n = s_merge[0], i0 = s_merge[1];
+              constexpr int WPC = CH == 8 ? 2 : 1;
+              float* half = reinterpret_cast<float*>(base + S::OFF_P);  // [16][128], the p operands are idle
+              for (int cb = 0; cb < cols; cb += 16 / WPC) {
+                const int c = cb + wi / WPC;
+                float sum = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (c < cols) sum = tree_add<WPC>(ta, CH, c, i0, n, wi % WPC, lane, hd, x);
+                if constexpr (WPC == 2) {
+                  if (wi & 1) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) half[wi * 128 + e * 32 + lane] = x[e];
+                  }
+                  group_sync(g);
+                  if (!(wi & 1)) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[e] += half[(wi + 1) * 128 + e * 32 + lane];
+                  }
+                }
+                if (c < cols && wi % WPC == 0) {
+#pragma unroll
+                  for (int e = 0; e < 4; e++)
+                    if (e * 32 + lane < hd) out_seq[col_off[set][c] + e * 32 + lane] = sum == 0.0f ? 0.0f : x[e] / sum;
+                }
+              }
+            }
+          }
         }
       }
       more = sg.more;
@@ -1108,7 +1190,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
 }
 
 // The units that several CTAs shared, each found at the CTA it began in: one
-// warp per column sums the partials in the order of the tiles.
+// warp per column.
 __global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__ TreeTcArgs ta, int ch) {
   const TreeArgs& a = ta.t;
   const int group = a.n_heads / a.c.n_kv, hd = a.c.hd, lane = threadIdx.x & 31;
@@ -1117,33 +1199,13 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__
   pdl_trigger();
   const TreePart u = ta.parts[i0];
   if (c >= ch || !u.n || c >= u.cols) return;
-  auto slot = [&](int i) { return (2 * (size_t)(i0 + i) + (i == 0 ? 1 : 0)) * ch + c; };
-  float m = -INFINITY;
-  for (int i = lane; i < u.n; i += 32) m = fmaxf(m, __ldcg(&ta.part_ml[slot(i)]).x);
-  m = warp_max(m);
-  float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int ib = 0; ib < u.n; ib += 32) {
-    float wt = 0.0f;
-    if (ib + lane < u.n) {
-      const float2 f = __ldcg(&ta.part_ml[slot(ib + lane)]);
-      wt = f.x == -INFINITY ? 0.0f : ex2(f.x - m);
-      l = fmaf(f.y, wt, l);
-    }
-#pragma unroll 8
-    for (int i = 0; i < min(32, u.n - ib); i++) {
-      const float f = __shfl_sync(0xffffffffu, wt, i);
-      const float* po = ta.part_o + slot(ib + i) * hd;
-#pragma unroll
-      for (int e = 0; e < 4; e++)
-        if (e * 32 + lane < hd) o[e] = fmaf(__ldcg(po + e * 32 + lane), f, o[e]);
-    }
-  }
-  l = warp_sum(l);
+  float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  const float sum = tree_add<1>(ta, ch, c, i0, u.n, 0, lane, hd, x);
   const int vh = u.vh0 + c, node = vh / group, head = u.kvh * group + vh % group;
   float* out = a.out + ((size_t)(u.off + node) * a.n_heads + head) * hd;
 #pragma unroll
   for (int e = 0; e < 4; e++)
-    if (e * 32 + lane < hd) out[e * 32 + lane] = l == 0.0f ? 0.0f : o[e] / l;
+    if (e * 32 + lane < hd) out[e * 32 + lane] = sum == 0.0f ? 0.0f : x[e] / sum;
 }
 
 static size_t al256(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -1154,7 +1216,7 @@ static int tt_columns(int max_nodes, int group) {
 
 size_t tree_workspace_bytes(int max_nodes, int n_heads, int n_kv, int hd, int sm_count) {
   const size_t cols = (size_t)2 * sm_count * tt_columns(max_nodes, n_heads / n_kv);
-  return al256(sm_count * sizeof(TreePart)) + al256(cols * 8) + al256(cols * hd * 4);
+  return al256(sm_count * sizeof(unsigned)) + al256(sm_count * sizeof(TreePart)) + al256(cols * 8) + al256(cols * hd * 4);
 }
 
 template <typename F>
@@ -1188,7 +1250,7 @@ static cudaError_t tt_go(TreeTcArgs& ta, cudaStream_t st) {
   if (ta.slots > TT_MAX_SLOTS) ta.slots = TT_MAX_SLOTS;
   void* args[] = {&ta};
   e = tt_launch(k, dim3(ta.t.sm_count), TT_THREADS, S::BYTES, st, args);
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess || S::TICKET) return e;
   int ch = S::CH;
   void* margs[] = {&ta, &ch};
   return tt_launch(tree_merge_kernel, dim3(ta.t.sm_count, S::CH / 4), 128, 0, st, margs);
@@ -1212,6 +1274,8 @@ cudaError_t launch_attn_tree(const TreeArgs& a, cudaStream_t st) {
   const int cols = tt_columns(a.max_nodes, group);
   const size_t n = (size_t)2 * a.sm_count * cols;
   uint8_t* w = static_cast<uint8_t*>(a.work);
+  ta.tickets = a.tickets ? a.tickets : reinterpret_cast<unsigned*>(w);
+  w += al256(a.sm_count * sizeof(unsigned));
   ta.parts = reinterpret_cast<TreePart*>(w);
   w += al256(a.sm_count * sizeof(TreePart));
   ta.part_ml = reinterpret_cast<float2*>(w);

@@ -56,7 +56,11 @@ def quantize_q8(rows: int, cols: int, w) -> tuple[np.ndarray, np.ndarray]:
 def synchronize(device: int | None = None) -> None:
     """Wait for this device's kernel-level calls; raises PranaError
     (PRANA_E_TIMEOUT) when a bounded device wait gave up in one of them."""
-    call("prana_ctx_synchronize", context(device))
+    try:
+        call("prana_ctx_synchronize", context(device))
+    except _ffi.PranaError:
+        _tree_work.clear()  # a kernel that gave up may have left its counters anywhere
+        raise
 
 
 def debug_wait_timeout(which: int, polls: int, device: int | None = None) -> int:
@@ -477,7 +481,7 @@ def attention_tree(q: torch.Tensor, cache: KvRows, starts: torch.Tensor, lens: t
     key = (index, _raw_stream(index))
     work = _tree_work.get(key)
     if work is None or work.numel() < size.value or _capturing():
-        work = torch.empty(size.value, dtype=torch.uint8, device=device)
+        work = torch.zeros(size.value, dtype=torch.uint8, device=device)  # its counters start at zero
         if not _capturing():  # a graph's memory belongs to the graph
             _tree_work[key] = work
     call("prana_attention_tree", ctx, q.data_ptr(), cache._ref, cache._int32(starts, (n_seq,), "starts"),
