@@ -6,6 +6,7 @@
 //   out = sum_j exp(s_j - max) v_j / sum_j exp(s_j - max)   (zeros: nothing seen)
 // A place that a node does not see takes no part, whatever it holds.
 #include <atomic>
+#include <climits>
 
 #include "internal.h"
 #include "mbar.cuh"
@@ -369,16 +370,15 @@ template <int STEP>
 __device__ __forceinline__ float tree_add(const TreeTcArgs& ta, int ch, int c, int i0, int n, int from, int lane, int hd,
                                           float (&x)[4]) {
   auto slot = [&](int i) { return (2 * (size_t)(i0 + i) + (i == 0 ? 1 : 0)) * ch + c; };
-  float m = -INFINITY, sum = 0.0f;
-  for (int i = lane; i < n; i += 32) m = fmaxf(m, __ldcg(&ta.part_ml[slot(i)]).x);
+  auto ml = [&](int i) { return i < n ? __ldcg(&ta.part_ml[slot(i)]) : make_float2(-INFINITY, 0.0f); };
+  float2 f0 = ml(lane);
+  float m = f0.x, sum = 0.0f;
+  for (int i = lane + 32; i < n; i += 32) m = fmaxf(m, ml(i).x);
   m = warp_max(m);
   for (int ib = 0; ib < n; ib += 32) {
-    float wt = 0.0f;
-    if (ib + lane < n) {
-      const float2 f = __ldcg(&ta.part_ml[slot(ib + lane)]);
-      wt = f.x == -INFINITY ? 0.0f : ex2(f.x - m);
-      sum = fmaf(f.y, wt, sum);
-    }
+    if (ib) f0 = ml(ib + lane);
+    const float wt = f0.x == -INFINITY ? 0.0f : ex2(f0.x - m);
+    sum = fmaf(f0.y, wt, sum);
 #pragma unroll 8
     for (int i = from; i < min(32, n - ib); i += STEP) {
       const float f = __shfl_sync(0xffffffffu, wt, i);
@@ -417,13 +417,14 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
   // a slot in turn when their number is odd, for two waiters: each has its own
   // `full`.)
   __shared__ __align__(8) uint64_t full[2][TT_MAX_SLOTS], empty[TT_MAX_SLOTS];  // full: of K, of V
-  __shared__ __align__(8) uint64_t s_full[4], s_free[4], p_full[4], o_full[4], q_ready, q_seen, q_free, done_s, done_o;
+  __shared__ __align__(8) uint64_t s_full[4], s_free[4], p_full[4], o_full[4], q_ready, q_seen, q_free, parts0, done_s, done_o;
   __shared__ uint32_t tmem_s;
   __shared__ int s_abort;
   // a segment and its columns, in one of two sets: the nodes a column's node sees,
   // its place in the sequence's q and out rows, its score factor; and the nodes
   // some column sees
   __shared__ TreeSegment seg_tab[2];
+  __shared__ int2 seg_part[2];  // the CTA where its unit began, and how many the unit went to
   __shared__ unsigned long long col_mask[2][CH], any_mask[2];
   __shared__ int col_off[2][CH];
   __shared__ __align__(16) float col_mul[2][CH];
@@ -463,6 +464,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
     mbar_init(&q_ready, 32);
     mbar_init(&q_free, 1);
     mbar_init(&q_seen, 1);
+    mbar_init(&parts0, 1);
     mbar_init(&done_s, 1);
     mbar_init(&done_o, 1);
     fence_barrier_init();
@@ -744,6 +746,22 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
     stage(seg_tab[0], 0, TT_SOFT / 32, TT_SOFT / 32 + 1);
     first_sync();
     mbar_arrive(&q_ready);
+    auto part = [&](const TreeSegment& sg) {
+      const unsigned shares = s_all < gridDim.x ? (unsigned)s_all : gridDim.x;
+      const int all = sg.before + sg.tiles + sg.rest;
+      auto cta = [&](unsigned long long place) {  // whose share holds it
+        const unsigned long long x = (place + 1) * shares - 1;
+        return x <= 0xffffffffull ? (int)((unsigned)x / (unsigned)s_all) : (int)(x / s_all);
+      };
+      // a unit that goes on ends this share, one that came from before began it
+      const unsigned long long u0 = sg.before ? s_all * blockIdx.x / shares - sg.before : s_all * (blockIdx.x + 1) / shares - sg.tiles;
+      const int i0 = cta(u0);
+      return make_int2(i0, cta(u0 + all - 1) - i0 + 1);
+    };
+    if (lane == 0) {
+      seg_part[0] = part(seg_tab[0]);
+      mbar_arrive(&parts0);
+    }
     TreeWalk w = s_walk;
     for (int seg = 1; w.next(); seg++) {
       const int set = seg & 1;
@@ -752,7 +770,10 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
       tt_wait(&q_free, (uint32_t)(seg - 1) & 1, abort);  // the last segment's products have read the operand
       if (*abort) break;
       const TreeSegment sg = tree_segment(w);
-      if (lane == 0) seg_tab[set] = sg;
+      if (lane == 0) {
+        seg_tab[set] = sg;
+        seg_part[set] = part(sg);
+      }
       stage(sg, set, 0, 1);
       mbar_arrive(&q_ready);
     }
@@ -1110,7 +1131,10 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
           for (int c = 0; c < NQ; c++)
             if (c0 + c < cols) put(c, x_fin[g][c].x, x_fin[g][c].y, c & 1 ? o[c / 2].hi() : o[c / 2].lo());
         } else {
-          for (int c = tg; c < NQ && c0 + c < cols; c += TG) {  // the teams share the columns
+#pragma unroll
+          for (int i = 0; i < NQ / TG; i++) {  // the teams share the columns
+            const int c = i * TG + tg;
+            if (c0 + c >= cols) break;
             float m = -INFINITY, sum = 0.0f, x = 0.0f;
 #pragma unroll
             for (int q = 0; q < TG; q++) m = fmaxf(m, x_fin[q * CG + cg][c].x);
@@ -1125,16 +1149,10 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
           }
         }
         if (!whole) {
-          if (S::TICKET) {
-            __threadfence();
-            groups_sync();
-          }
+          if (S::TICKET) groups_sync();
           if (tid == 0) {
-            // the unit's tiles among all places, and the CTAs they went to
-            const unsigned long long shares = s_all < gridDim.x ? s_all : gridDim.x;
-            const int all = sg.before + tiles + sg.rest;
-            const unsigned long long u0 = first_part ? s_all * (blockIdx.x + 1) / shares - tiles : s_all * blockIdx.x / shares - sg.before;
-            const int i0 = (int)(((u0 + 1) * shares - 1) / s_all), n = (int)(((u0 + all) * shares - 1) / s_all) - i0 + 1;
+            if (seg_no == 0) tt_wait(&parts0, 0, abort);
+            const int i0 = seg_part[set].x, n = seg_part[set].y;
             if constexpr (S::TICKET) {
               const bool last = ticket_acq_rel(ta.tickets + i0) == (unsigned)n - 1;
               if (last) ta.tickets[i0] = 0u;
@@ -1209,13 +1227,18 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__
 }
 
 static size_t al256(size_t x) { return (x + 255) & ~(size_t)255; }
-static int tt_columns(int max_nodes, int group) {
+// Columns of a CTA: as many as there are, up to 64, so that the cache is read
+// once.  33 to 64 of a few units are taken as two chunks of 32: with two tiles
+// or so for each SM, two teams and no merge kernel count for more than reading
+// twice (16 nodes x 4 heads over 4096 f16 positions, 8 kv heads: one sequence 29 us
+// against 36; four of 3000 46 against 43).
+static int tt_columns(int max_nodes, int group, int units) {
   const int vh = max_nodes * group;
-  return vh <= 8 ? 8 : vh <= 16 ? 16 : vh <= 32 ? 32 : 64;
+  return vh <= 8 ? 8 : vh <= 16 ? 16 : vh <= 32 || (vh <= 64 && units <= 16) ? 32 : 64;
 }
 
 size_t tree_workspace_bytes(int max_nodes, int n_heads, int n_kv, int hd, int sm_count) {
-  const size_t cols = (size_t)2 * sm_count * tt_columns(max_nodes, n_heads / n_kv);
+  const size_t cols = (size_t)2 * sm_count * tt_columns(max_nodes, n_heads / n_kv, INT_MAX);
   return al256(sm_count * sizeof(unsigned)) + al256(sm_count * sizeof(TreePart)) + al256(cols * 8) + al256(cols * hd * 4);
 }
 
@@ -1271,7 +1294,7 @@ cudaError_t launch_attn_tree(const TreeArgs& a, cudaStream_t st) {
   }
   ta.t = a;
   ta.boxes = !c.q8 && c.hd > 64 ? 2 : 1;
-  const int cols = tt_columns(a.max_nodes, group);
+  const int cols = tt_columns(a.max_nodes, group, a.n_seq > 16 ? INT_MAX : a.n_seq * c.n_kv);
   const size_t n = (size_t)2 * a.sm_count * cols;
   uint8_t* w = static_cast<uint8_t*>(a.work);
   ta.tickets = a.tickets ? a.tickets : reinterpret_cast<unsigned*>(w);
