@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(TR_THREADS) tree_simple_kernel(const TreeArgs 
 //
 // Exactness.  An f16 cache: q and p enter as f16 head + remainder pairs (22
 // bits), K and V as they are, sums in f32.  An int8 cache: q enters as three signed
-// base-256 digits (23 bits), p as four (31), and kind::i8 products take K and V as
+// base-256 digits (23 bits), p as two pairs (30), and kind::i8 products take K and V as
 // they lie in memory, with no conversion; every product and sum is an exact
 // integer (a digit's sum over a tile stays within 2^21).  The K scale multiplies
 // the score in f32.  The V scale, 2^e * m, goes with the probability: e is added to
@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(TR_THREADS) tree_simple_kernel(const TreeArgs 
 //   The reference of a column is its largest score when it was last set; it
 // is set at the first tile, at tiles with drafted places, and when a later score
 // passes it by more than TT_ROOM powers of two, which the digits and the f16 range
-// have to spare (p = 1 keeps 26 bits).  Until then O gathers in TMEM over the
+// have to spare (p = 1 keeps 23 bits).  Until then O gathers in TMEM over the
 // tiles, and a tile needs no maximum, no exchange and no rescaling.
 //
 // Roles (20 warps): 16 loads K and V tiles by TMA into a ring of slots, 17 issues
@@ -140,13 +140,19 @@ constexpr int TT_TMA_WARP = 16, TT_S_WARP = 17, TT_O_WARP = 18, TT_Q_WARP = 19;
 constexpr int TT_TILE = 128;
 constexpr int TT_MAX_SLOTS = 10;
 constexpr float TT_DIGITS = 8355711.0f;  // 0x7f7f7f: the largest value of three balanced digits
-constexpr float TT_ROOM = 8.0f;
-// Units of the p operand for p = 1 (with m < 2): 2^4 * 2 of them stay below
-// 0x7f7f7f7f, the largest value of four digits, 2^4 * 2^11 below f16's largest.
+constexpr float TT_ROOM = 6.0f;
+// Units of the p operand for p = 1 (with m < 2): 2^6 * 2 of them stay below 2^15 *
+// 0x7f7f, the largest value of its digits, 2^6 * 2^9 below f16's largest.
+// Room for 2^8 rescaled less often (24 trees of 60 nodes 594 us, 617 with 2^4) but
+// lost two digits' worth of the f32 sums' accuracy (1.5e-6 against 6e-7).
 template <bool Q8>
-constexpr float TT_UNITS = Q8 ? 2139000000.0f / 512.0f : 128.0f;
-// Tiles that O may gather: 2^21 x 512 fits 32 bits
-constexpr int TT_RUN = 512;
+constexpr float TT_UNITS = Q8 ? 1069500000.0f / 128.0f : 512.0f;
+// Tiles that O may gather.  Digits: 2^21 x 512 fits 32 bits.  f32: none beyond
+// the tile, since the tensor core cuts sums off where it does not round them
+// (66000 positions: an error of 4.8e-6 with 31 tiles, 2.0e-6 with four, 6.5e-7 with
+// one, at no cost in time).
+template <bool Q8>
+constexpr int TT_RUN = Q8 ? 512 : 1;
 constexpr float LOG2E = 1.4426950408889634f;
 
 // What a CTA leaves for tree_merge_kernel: the unit that began in it and went on
@@ -848,9 +854,9 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
             for (int c = 0; c < 8; c += 2) {
               F2& x = o[(cb + c) / 2];
               if constexpr (Q8) {
-                const F2 k(256.0f);
+                const F2 k(256.0f), k7(128.0f);
                 auto digit = [&](int z) { return F2((float)(int)v[8 * z + c], (float)(int)v[8 * z + c + 1]); };
-                x = fma2(fma2(fma2(fma2(digit(0), k, digit(1)), k, digit(2)), k, digit(3)), unit, x);
+                x = fma2(fma2(fma2(fma2(digit(0), k, digit(1)), k7, digit(2)), k, digit(3)), unit, x);
               } else {
                 x = fma2(joined<false, 8>(v, c), unit, x);
               }
@@ -938,7 +944,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
         }
         // tiles with drafted places set the references anew each: whether another
         // node's score passes its reference must not touch this one's sums
-        bool fresh = run == 0 || run == TT_RUN || (edge && trees);
+        bool fresh = run == 0 || (edge && trees);
         if (run) {
           float top = -INFINITY;
 #pragma unroll
@@ -987,6 +993,9 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
             o[c / 2 + 1] = o[c / 2 + 1] * F2(al.z, al.w);
           }
           run = 0;
+        } else if (held && run % TT_RUN<Q8> == 0) {
+          fold();
+          held = false;
         }
         // ---- probabilities, in the operand's form, a row per position
         if constexpr (Q8) {
@@ -1003,14 +1012,17 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
             const F2 p0(ex2(s[c / 2].lo()), ex2(s[c / 2].hi())), p1(ex2(s[c / 2 + 1].lo()), ex2(s[c / 2 + 1].hi()));
             l[c / 2] = fma2(p0, iv, l[c / 2]);
             l[c / 2 + 1] = fma2(p1, iv, l[c / 2 + 1]);
-            const F2 f0 = p0 * cm, f1 = p1 * cm;
-            // balanced digits: bytes of the value + 0x808080, the lower three less 128
-            const uint32_t f[4] = {(uint32_t)__float2int_rn(f0.lo()) + 0x808080u, (uint32_t)__float2int_rn(f0.hi()) + 0x808080u,
-                                   (uint32_t)__float2int_rn(f1.lo()) + 0x808080u, (uint32_t)__float2int_rn(f1.hi()) + 0x808080u};
-            const uint32_t a01 = __byte_perm(f[0], f[1], 0x5140), a23 = __byte_perm(f[2], f[3], 0x5140);
-            const uint32_t b01 = __byte_perm(f[0], f[1], 0x7362), b23 = __byte_perm(f[2], f[3], 0x7362);
+            // x = 2^15 h + l, both by adding 3 * 2^22 (and 128, which makes the lower byte's
+            // balanced digit that byte less 128): two digits each, all exact
+            const F2 x0 = p0 * cm, x1 = p1 * cm, one(12582912.0f + 128.0f), low(-32768.0f);
+            const F2 h0 = fma2(x0, F2(1.0f / 32768.0f), one), h1 = fma2(x1, F2(1.0f / 32768.0f), one);
+            const F2 minus(-12582912.0f - 128.0f);
+            const F2 l0 = fma2(h0 + minus, low, x0) + one, l1 = fma2(h1 + minus, low, x1) + one;
+            auto word = [](float x) { return __float_as_uint(x); };
+            const uint32_t a01 = __byte_perm(word(l0.lo()), word(l0.hi()), 0x5140), a23 = __byte_perm(word(l1.lo()), word(l1.hi()), 0x5140);
+            const uint32_t b01 = __byte_perm(word(h0.lo()), word(h0.hi()), 0x5140), b23 = __byte_perm(word(h1.lo()), word(h1.hi()), 0x5140);
             dg[3][c / 4] = __byte_perm(a01, a23, 0x5410) ^ 0x80808080u;
-            dg[2][c / 4] = __byte_perm(a01, a23, 0x7632) ^ 0x80808080u;
+            dg[2][c / 4] = __byte_perm(a01, a23, 0x7632);
             dg[1][c / 4] = __byte_perm(b01, b23, 0x5410) ^ 0x80808080u;
             dg[0][c / 4] = __byte_perm(b01, b23, 0x7632);
           }
