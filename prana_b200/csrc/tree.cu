@@ -127,8 +127,8 @@ __global__ void __launch_bounds__(TR_THREADS) tree_simple_kernel(const TreeArgs 
 //
 // Roles (20 warps): 16 loads K and V tiles by TMA into a ring of slots, 17 issues
 // S = K . q^T (M = 128 positions), 18 issues O^T = V^T . p^T (M = dims; V is read
-// MN-major as it lies, p is written position by position), 19 prepares the next
-// segment's columns, and four groups of four warps do the softmax, a thread per
+// MN-major as it lies, p is written position by position), 19 finds the
+// next segment and prepares its columns, and four groups of four warps do the softmax, a thread per
 // position for S and a thread per dim for O, 16 columns at most.  The groups form
 // teams with a tile each: up to 16 columns four teams of one group, with 32 two
 // teams of two, with 64 one team of four, whose columns share one product.  (A
@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(TR_THREADS) tree_simple_kernel(const TreeArgs 
 // columns and 100 at 192: four of 48 took twice one of 192.)  The cache is so read
 // once for 64 columns.
 constexpr int TT_GROUPS = 4, TT_SOFT = TT_GROUPS * 128, TT_THREADS = TT_SOFT + 128;
-constexpr int TT_TMA_WARP = 16, TT_S_WARP = 17, TT_O_WARP = 18, TT_Q_WARP = 19;
+constexpr int TT_TMA_WARP = 16, TT_S_WARP = 17, TT_O_WARP = 18, TT_NEXT_WARP = 19;
 constexpr int TT_TILE = 128;
 constexpr int TT_MAX_SLOTS = 10;
 constexpr float TT_DIGITS = 8355711.0f;  // 0x7f7f7f: the largest value of three balanced digits
@@ -190,8 +190,17 @@ struct TtShape {
   // that time (600 KB of a 4096 context), and a kernel follows.
   static constexpr bool TICKET = CH <= 32;
   static_assert(TG * (CS + CO) <= 512, "TMEM");
-  // a segment's start and end, in tiles (8 to 14 thousand cycles against 1.5 of a decode tile, 4 of a wide one)
-  static constexpr int LEAD = CG == 1 ? 4 : 2;
+  // Warps that prepare the next segment's columns.  Up to 16, one warp does while
+  // the segment before ends (given to the softmax warps it made 24 sequences' decode 15%
+  // slower).  More are a chain of 8 or 16 trips to memory for that warp, which
+  // nothing hides (15 us for 64 columns): the softmax warps do them, one trip each
+  // (24 trees of 60 nodes 540 -> 485 us).
+  static constexpr int STAGERS = CG == 1 ? 1 : TT_SOFT / 32;
+  // A segment's start and end, in tiles: 7 to 10 us against 2 of a wide tile, 3 against
+  // 0.9 of a decode tile.  (24 sequences of 6000, int8, are 2% slower with 2 and the
+  // same from 4 to 10; 24 trees of 60 nodes over 6000 f16 positions 495 us with 2, 462
+  // with 4, 434 with 8, but eight trees over 1000, int8, 70, 70 and 75.)
+  static constexpr int LEAD = 4;
   static_assert(TG == 1 || PSZ >= CG * NQ * 128 * 4, "the groups' o pass through the p operand");
 };
 
@@ -283,7 +292,7 @@ __device__ __forceinline__ bool team_any(int team, bool pred) {
       : "memory");
   return r != 0;
 }
-__device__ __forceinline__ void first_sync() { asm volatile("bar.sync 6, 544;" ::: "memory"); }  // the groups and the column warp
+__device__ __forceinline__ void first_sync() { asm volatile("bar.sync 6, 544;" ::: "memory"); }  // the groups and the next segments' warp
 __device__ __forceinline__ void groups_sync() { asm volatile("bar.sync 5, 512;" ::: "memory"); }
 __device__ __forceinline__ bool groups_any(bool pred) {
   uint32_t r;
@@ -423,7 +432,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
   // a slot in turn when their number is odd, for two waiters: each has its own
   // `full`.)
   __shared__ __align__(8) uint64_t full[2][TT_MAX_SLOTS], empty[TT_MAX_SLOTS];  // full: of K, of V
-  __shared__ __align__(8) uint64_t s_full[4], s_free[4], p_full[4], o_full[4], q_ready, q_seen, q_free, parts0, done_s, done_o;
+  __shared__ __align__(8) uint64_t s_full[4], s_free[4], p_full[4], o_full[4], q_ready, q_free, seg_seen, seg_ready, parts0, done_s, done_o;
   __shared__ uint32_t tmem_s;
   __shared__ int s_abort;
   // a segment and its columns, in one of two sets: the nodes a column's node sees,
@@ -467,9 +476,10 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
       mbar_init(&p_full[g], 128 * CG);
       mbar_init(&o_full[g], 1);
     }
-    mbar_init(&q_ready, 32);
+    mbar_init(&q_ready, 32 * S::STAGERS);
     mbar_init(&q_free, 1);
-    mbar_init(&q_seen, 1);
+    mbar_init(&seg_seen, 1);
+    mbar_init(&seg_ready, 1);
     mbar_init(&parts0, 1);
     mbar_init(&done_s, 1);
     mbar_init(&done_o, 1);
@@ -747,11 +757,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
       if (!mbar_wait(last, 0, *abort ? 1u << 16 : kMbarPolls)) *abort = 1;
     }
     __syncwarp();
-  } else if (wi == TT_Q_WARP) {
-    // ------------------------------------------------ the next segment's columns: q operand, masks, places
-    stage(seg_tab[0], 0, TT_SOFT / 32, TT_SOFT / 32 + 1);
-    first_sync();
-    mbar_arrive(&q_ready);
+  } else if (wi == TT_NEXT_WARP) {
+    // ------------------------------------------------ the segments, one ahead
     auto part = [&](const TreeSegment& sg) {
       const unsigned shares = s_all < gridDim.x ? (unsigned)s_all : gridDim.x;
       const int all = sg.before + sg.tiles + sg.rest;
@@ -764,6 +771,9 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
       const int i0 = cta(u0);
       return make_int2(i0, cta(u0 + all - 1) - i0 + 1);
     };
+    stage(seg_tab[0], 0, TT_SOFT / 32, TT_SOFT / 32 + 1);
+    first_sync();
+    if (S::STAGERS == 1) mbar_arrive(&q_ready);
     if (lane == 0) {
       seg_part[0] = part(seg_tab[0]);
       mbar_arrive(&parts0);
@@ -772,16 +782,19 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
     for (int seg = 1; w.next(); seg++) {
       const int set = seg & 1;
       // everybody is in the last segment, so the set's readers, two segments ago, are done
-      tt_wait(&q_seen, (uint32_t)(seg - 1) & 1, abort);
-      tt_wait(&q_free, (uint32_t)(seg - 1) & 1, abort);  // the last segment's products have read the operand
-      if (*abort) break;
+      tt_wait(&seg_seen, (uint32_t)(seg - 1) & 1, abort);
+      if (S::STAGERS == 1) tt_wait(&q_free, (uint32_t)(seg - 1) & 1, abort);  // the last segment's products have read q
+      if (__any_sync(0xffffffffu, *abort != 0)) break;
       const TreeSegment sg = tree_segment(w);
       if (lane == 0) {
         seg_tab[set] = sg;
         seg_part[set] = part(sg);
+        if (S::STAGERS > 1) mbar_arrive(&seg_ready);
       }
-      stage(sg, set, 0, 1);
-      mbar_arrive(&q_ready);
+      if constexpr (S::STAGERS == 1) {
+        stage(sg, set, 0, 1);
+        mbar_arrive(&q_ready);
+      }
     }
   } else {
     // ------------------------------------------------ softmax groups
@@ -797,12 +810,12 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
     do {
       const int set = seg_no & 1;
       if (seg_no) {
-        tt_wait(&q_ready, (uint32_t)seg_no & 1, abort);  // the segment and its columns' tables
+        tt_wait(&q_ready, (uint32_t)seg_no & 1, abort);  // its columns' tables
         // one decision for all, so that the named barriers stay matched; from here
         // on the last segment's p operands are free
         if (groups_any(*abort != 0)) break;
       }
-      if (tid == 0) mbar_arrive(&q_seen);
+      if (tid == 0) mbar_arrive(&seg_seen);
       const TreeSegment& sg = seg_tab[set];
       const int len = sg.len, total = sg.total, tiles = sg.tiles;
       const int first = (tg - k0) & (TG - 1);
@@ -822,9 +835,10 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
         vs_at = a.c.v_scale + at;
         scales(first);
       }
-      if (seg_no == 0) {  // the first segment's columns are everybody's work
+      if (seg_no == 0) {
         stage(sg, 0, wi, TT_SOFT / 32 + 1);
         first_sync();
+        if (S::STAGERS > 1) mbar_arrive(&q_ready);
       }
       F2 l[NQ / 2], o[NQ / 2];
       float ref = -INFINITY;  // lane c: the reference of column c; none yet
@@ -1087,6 +1101,13 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
         run++;
         fence_async_smem();
         mbar_arrive(&p_full[tg]);
+      }
+      if (S::STAGERS > 1 && sg.more) {
+        // the next segment's columns, so that its scores are under way while this one ends
+        tt_wait(&seg_ready, (uint32_t)seg_no & 1, abort);
+        tt_wait(&q_free, (uint32_t)seg_no & 1, abort);  // this segment's products have read the operand
+        if (!__any_sync(0xffffffffu, *abort != 0)) stage(seg_tab[set ^ 1], set ^ 1, wi, TT_SOFT / 32);
+        mbar_arrive(&q_ready);
       }
       if (held) fold();
       if constexpr (!Q8) {  // drafted rows of V that are not finite: nodes that see them get NaN
