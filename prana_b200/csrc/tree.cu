@@ -268,6 +268,13 @@ __device__ __forceinline__ F2 joined(const uint32_t* v, int c) {
 // Each try may suspend for 20 us: a spinning warp takes issue slots from the rest.
 constexpr uint32_t TT_POLLS = 1u << 17;
 __device__ __forceinline__ void tt_wait(uint64_t* bar, uint32_t phase, volatile int* abort) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(phase)
+      : "memory");
+  if (done) return;
   for (uint32_t i = 0; i < TT_POLLS; i++) {
     uint32_t ok;
     asm volatile(
