@@ -264,17 +264,18 @@ __device__ __forceinline__ F2 joined(const uint32_t* v, int c) {
   }
 }
 // A bounded wait.  Once any role of the CTA has given up, every wait returns at
-// once: the loops run on to their ends, so that named barriers stay matched.
-// Each try may suspend for 20 us: a spinning warp takes issue slots from the rest.
+// once: the loops run on to their ends, so that named barriers stay matched.  A
+// try may suspend, for 20 us at most, since a spinning warp takes issue slots from
+// the rest; it takes 350 cycles even for a phase long over, a test 150, so that
+// comes first, `LOOKS` times.
 constexpr uint32_t TT_POLLS = 1u << 17;
-__device__ __forceinline__ void tt_wait(uint64_t* bar, uint32_t phase, volatile int* abort) {
-  uint32_t done;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-      : "=r"(done)
-      : "r"(smem_u32(bar)), "r"(phase)
-      : "memory");
-  if (done) return;
+constexpr int TT_LOOKS = 1;  // of the roles that issue copies and products
+template <int LOOKS = 1>
+__device__ __forceinline__ bool tt_wait(uint64_t* bar, uint32_t phase, volatile int* abort) {
+#pragma unroll 1
+  for (int i = 0; i < LOOKS; i++)
+    if (mbar_test_wait(bar, phase)) return true;
+#pragma unroll 1
   for (uint32_t i = 0; i < TT_POLLS; i++) {
     uint32_t ok;
     asm volatile(
@@ -282,10 +283,11 @@ __device__ __forceinline__ void tt_wait(uint64_t* bar, uint32_t phase, volatile 
         : "=r"(ok)
         : "r"(smem_u32(bar)), "r"(phase), "r"(20000u)
         : "memory");
-    if (ok) return;
-    if (*abort) return;
+    if (ok) return true;
+    if (*abort) return false;
   }
   *abort = 1;
+  return false;
 }
 __device__ __forceinline__ void group_sync(int g) { asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory"); }
 // the OR of `pred` over the 128 * N threads of a team (barriers 7 and up)
@@ -492,6 +494,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
     mbar_init(&done_o, 1);
     fence_barrier_init();
   }
+  if (tid == 32 || tid == 64)
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(tid == 32 ? &ta.tm_k : &ta.tm_v)) : "memory");
   __syncthreads();
   pdl_wait();     // what comes next reads what earlier kernels wrote
   pdl_trigger();  // the merge kernel may take its place; it waits for this grid
@@ -664,8 +668,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
       do {
         for (int t = w.tile; go && t < w.tile + w.seg; t++)
           for (int kv = 0; kv < 2; kv++) {
-            tt_wait(&empty[slot], phase, abort);
-            if (*abort) {
+            if (!tt_wait<TT_LOOKS>(&empty[slot], phase, abort)) {
               go = false;
               break;
             }
@@ -696,14 +699,13 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
       uint32_t phase = 0, segs = 0;
       int turn = 0;  // of `period` tiles, after which a slot's barrier is in its next phase
       bool fresh = true;  // a segment begins: its columns first
-      for (int k = 0; !*abort; k++) {
+      for (int k = 0;; k++) {
         const int g = k % TG;
         const uint32_t n = (uint32_t)(k / TG);
         if (scores) {
-          if (fresh) tt_wait(&q_ready, segs & 1, abort);
-          if (n) tt_wait(&s_free[g], (n - 1) & 1, abort);
-          tt_wait(&full[scores ? 0 : 1][slot], phase, abort);
-          if (*abort) break;
+          if (fresh && !tt_wait(&q_ready, segs & 1, abort)) break;
+          if (n && !tt_wait<TT_LOOKS>(&s_free[g], (n - 1) & 1, abort)) break;
+          if (!tt_wait<TT_LOOKS>(&full[0][slot], phase, abort)) break;
           tc_fence_after();
           const uint64_t kd = sw128_desc(smem_u32(base + slot * slot_bytes));
           const uint64_t qd = sw128_desc(smem_u32(q_t));
@@ -725,9 +727,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
             segs++;
           }
         } else {
-          tt_wait(&p_full[g], n & 1, abort);
-          tt_wait(&full[scores ? 0 : 1][slot], phase, abort);
-          if (*abort) break;
+          if (!tt_wait<TT_LOOKS>(&p_full[g], n & 1, abort)) break;
+          if (!tt_wait<TT_LOOKS>(&full[1][slot], phase, abort)) break;
           tc_fence_after();
           // one 128-byte-wide block of M per box; a lone f16 box stands for both
           // halves (the upper half of O is not read)
