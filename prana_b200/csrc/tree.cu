@@ -267,15 +267,10 @@ __device__ __forceinline__ F2 joined(const uint32_t* v, int c) {
 // once: the loops run on to their ends, so that named barriers stay matched.  A
 // try may suspend, for 20 us at most, since a spinning warp takes issue slots from
 // the rest; it takes 350 cycles even for a phase long over, a test 150, so that
-// comes first, `LOOKS` times.
+// comes first (three of them are slower again).
 constexpr uint32_t TT_POLLS = 1u << 17;
-constexpr int TT_LOOKS = 1;  // of the roles that issue copies and products
-template <int LOOKS = 1>
 __device__ __forceinline__ bool tt_wait(uint64_t* bar, uint32_t phase, volatile int* abort) {
-#pragma unroll 1
-  for (int i = 0; i < LOOKS; i++)
-    if (mbar_test_wait(bar, phase)) return true;
-#pragma unroll 1
+  if (mbar_test_wait(bar, phase)) return true;
   for (uint32_t i = 0; i < TT_POLLS; i++) {
     uint32_t ok;
     asm volatile(
@@ -470,28 +465,29 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
   const uint32_t slot_bytes = (uint32_t)boxes * 16384u;
   const int period = slots & 1 ? slots : slots / 2;  // tiles between two uses of a slot by K (or by V)
 
-  if (tid == 0) {
-    s_abort = 0;
-    s_any = 0;
-    any_mask[0] = any_mask[1] = 0ull;
-    for (int i = 0; i < slots; i++) {
-      mbar_init(&full[0][i], 1);
-      mbar_init(&full[1][i], 1);
-      mbar_init(&empty[i], 1);
+  if (tid < 32) {
+    auto init = [&](uint64_t* bars, int n, unsigned count) {
+      if (lane < n) mbar_init(bars + lane, count);
+    };
+    init(full[0], TT_MAX_SLOTS, 1);
+    init(full[1], TT_MAX_SLOTS, 1);
+    init(empty, TT_MAX_SLOTS, 1);
+    init(s_full, TG, 1);
+    init(s_free, TG, 128 * CG);
+    init(p_full, TG, 128 * CG);
+    init(o_full, TG, 1);
+    if (lane == 0) {
+      s_abort = 0;
+      s_any = 0;
+      any_mask[0] = any_mask[1] = 0ull;
+      mbar_init(&q_ready, 32 * S::STAGERS);
+      mbar_init(&q_free, 1);
+      mbar_init(&seg_seen, 1);
+      mbar_init(&seg_ready, 1);
+      mbar_init(&parts0, 1);
+      mbar_init(&done_s, 1);
+      mbar_init(&done_o, 1);
     }
-    for (int g = 0; g < TG; g++) {
-      mbar_init(&s_full[g], 1);
-      mbar_init(&s_free[g], 128 * CG);
-      mbar_init(&p_full[g], 128 * CG);
-      mbar_init(&o_full[g], 1);
-    }
-    mbar_init(&q_ready, 32 * S::STAGERS);
-    mbar_init(&q_free, 1);
-    mbar_init(&seg_seen, 1);
-    mbar_init(&seg_ready, 1);
-    mbar_init(&parts0, 1);
-    mbar_init(&done_s, 1);
-    mbar_init(&done_o, 1);
     fence_barrier_init();
   }
   if (tid == 32 || tid == 64)
@@ -668,7 +664,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
       do {
         for (int t = w.tile; go && t < w.tile + w.seg; t++)
           for (int kv = 0; kv < 2; kv++) {
-            if (!tt_wait<TT_LOOKS>(&empty[slot], phase, abort)) {
+            if (!tt_wait(&empty[slot], phase, abort)) {
               go = false;
               break;
             }
@@ -704,8 +700,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
         const uint32_t n = (uint32_t)(k / TG);
         if (scores) {
           if (fresh && !tt_wait(&q_ready, segs & 1, abort)) break;
-          if (n && !tt_wait<TT_LOOKS>(&s_free[g], (n - 1) & 1, abort)) break;
-          if (!tt_wait<TT_LOOKS>(&full[0][slot], phase, abort)) break;
+          if (n && !tt_wait(&s_free[g], (n - 1) & 1, abort)) break;
+          if (!tt_wait(&full[0][slot], phase, abort)) break;
           tc_fence_after();
           const uint64_t kd = sw128_desc(smem_u32(base + slot * slot_bytes));
           const uint64_t qd = sw128_desc(smem_u32(q_t));
@@ -727,8 +723,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
             segs++;
           }
         } else {
-          if (!tt_wait<TT_LOOKS>(&p_full[g], n & 1, abort)) break;
-          if (!tt_wait<TT_LOOKS>(&full[1][slot], phase, abort)) break;
+          if (!tt_wait(&p_full[g], n & 1, abort)) break;
+          if (!tt_wait(&full[1][slot], phase, abort)) break;
           tc_fence_after();
           // one 128-byte-wide block of M per box; a lone f16 box stands for both
           // halves (the upper half of O is not read)
