@@ -267,10 +267,12 @@ __device__ __forceinline__ F2 joined(const uint32_t* v, int c) {
 // once: the loops run on to their ends, so that named barriers stay matched.  A
 // try may suspend, for 20 us at most, since a spinning warp takes issue slots from
 // the rest; it takes 350 cycles even for a phase long over, a test 150, so that
-// comes first (three of them are slower again).
+// comes first (three of them are slower again).  The loop stays
+// rolled: there are many waits, and the roles' loops lose 15% to instruction fetch.
 constexpr uint32_t TT_POLLS = 1u << 17;
 __device__ __forceinline__ bool tt_wait(uint64_t* bar, uint32_t phase, volatile int* abort) {
   if (mbar_test_wait(bar, phase)) return true;
+#pragma unroll 1
   for (uint32_t i = 0; i < TT_POLLS; i++) {
     uint32_t ok;
     asm volatile(
@@ -974,8 +976,12 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
           }
           if (!fresh) fresh = team_any<CG>(tg, top > TT_ROOM);
         }
+        if (held && (fresh || run % TT_RUN<Q8> == 0)) {
+          fold();
+          held = false;
+        }
         if (fresh) {
-          // ---- what O holds, then the references: a column's largest score so far
+          // ---- the references: a column's largest score so far
 #pragma unroll
           for (int c = 0; c < NQ; c += 4) {
             float4 m;
@@ -986,8 +992,6 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
             if (lane == 0) *reinterpret_cast<float4*>(&x_max[g][wq][c]) = m;
           }
           group_sync(g);
-          if (held) fold();
-          held = false;
           if (lane < NQ) {
             // against the old reference, or against 0 where there is none
             const float m = fmaxf(fmaxf(x_max[g][0][lane], x_max[g][1][lane]), fmaxf(x_max[g][2][lane], x_max[g][3][lane]));
@@ -1011,9 +1015,6 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
             o[c / 2 + 1] = o[c / 2 + 1] * F2(al.z, al.w);
           }
           run = 0;
-        } else if (held && run % TT_RUN<Q8> == 0) {
-          fold();
-          held = false;
         }
         // ---- probabilities, in the operand's form, a row per position
         if constexpr (Q8) {
