@@ -199,10 +199,11 @@ int prana_attention(prana_ctx *ctx, const float *q, const float *k, const float 
  * element strides (the last dimension is contiguous), as f16 or as int8 with
  * one f32 scale per position and head, [positions, n_kv_heads] with strides of
  * its own: value = q * scale.  head_dim is at most 256.  One such cache may hold
- * the rows of many sequences; row indexes, starts, lengths, paths and masks are
- * DEVICE arrays.  What they hold is checked on the device: a row or a sequence
- * that does not fit is left out, and the next prana_ctx_synchronize returns
- * PRANA_E_INVALID, once.  Calls never synchronize. */
+ * the rows of many sequences; attention streams int8 rows fastest where one
+ * head's positions are adjacent (row_stride = head_dim).  Row indexes, starts,
+ * lengths, paths and masks are DEVICE arrays.  What they hold is checked on the
+ * device: a row or a sequence that does not fit is left out, and the next
+ * prana_ctx_synchronize returns PRANA_E_INVALID, once.  Calls never synchronize. */
 #define PRANA_KV_F16 0
 #define PRANA_KV_Q8 1
 typedef struct prana_kv_rows {

@@ -201,6 +201,10 @@ struct TtShape {
   // same from 4 to 10; 24 trees of 60 nodes over 6000 f16 positions 495 us with 2, 462
   // with 4, 434 with 8, but eight trees over 1000, int8, 70, 70 and 75.)
   static constexpr int LEAD = 4;
+  // tiles until V is in the same slot again; a group that waits for its V knows that
+  // of its last tile has landed, and so all before
+  static constexpr int turn(int slots) { return slots & 1 ? slots : slots / 2; }
+  static_assert(turn(RING / 32768) >= TG && turn(RING / 16384 < TT_MAX_SLOTS ? RING / 16384 : TT_MAX_SLOTS) >= TG, "V's phases");
   static_assert(TG == 1 || PSZ >= CG * NQ * 128 * 4, "the groups' o pass through the p operand");
 };
 

@@ -346,6 +346,25 @@ def test_rows_past_32_bit_offsets(gpu, kind, n_kv, hd):
     b.check()
 
 
+def test_rows_past_32_bit_offsets_position_by_position(gpu):
+    n_kv, hd = 8, 128
+    positions = (1 << 31) // (n_kv * hd) + 1000
+    k, v = (torch.zeros((positions, n_kv, hd), dtype=torch.int8, device="cuda") for _ in range(2))
+    scales = torch.zeros((2, positions, n_kv), device="cuda")
+    b = Batch("q8", 2 * n_kv, n_kv, hd, lens=[700], nodes=[6], gap=0)
+    cache, first = K.KvRows(k, v, scales[0], scales[1]), positions - 706
+    rows, x = torch.arange(706, dtype=torch.int32, device="cuda"), torch.randn(706, n_kv, hd, device="cuda")
+    small = K.KvRows.alloc(706, n_kv, hd)
+    for c, at in ((small, 0), (cache, first)):
+        K.kv_rows_write(c, rows + at, x, x * 2)
+    for got, want in zip(K.kv_rows_read(cache, rows + first), K.kv_rows_read(small, rows)):
+        assert torch.equal(got, want)
+    for name in ("k", "v", "k_scale", "v_scale"):
+        getattr(cache, name)[first:] = getattr(b.cache, name)[:706]
+    b.cache, b.starts = cache, [first]
+    b.check()
+
+
 @pytest.mark.parametrize("kind", ["q8", "f16"])
 @pytest.mark.parametrize("hd", [64, 100])
 def test_sequences_that_do_not_fit_are_left_out_and_reported(gpu, kind, hd):
