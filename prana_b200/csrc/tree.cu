@@ -108,7 +108,8 @@ __global__ void __launch_bounds__(TR_THREADS) tree_simple_kernel(const TreeArgs 
 // chunk of columns), its tiles are 128 positions each, and the tiles of all
 // units, in order, are dealt to the CTAs (one per SM) in equal contiguous
 // shares, so ragged batches stay balanced.  A unit inside one share is finished
-// there; otherwise its shares leave (max, sum, o) partials for tree_merge_kernel.
+// there; otherwise its shares leave (max, sum, o) partials, which the CTA that is
+// done last adds up, or tree_merge_kernel where there are 64 columns.
 //
 // Exactness.  An f16 cache: q and p enter as f16 head + remainder pairs (22
 // bits), K and V as they are, sums in f32.  An int8 cache: q enters as three signed
@@ -122,19 +123,28 @@ __global__ void __launch_bounds__(TR_THREADS) tree_simple_kernel(const TreeArgs 
 //   The reference of a column is its largest score when it was last set; it
 // is set at the first tile, at tiles with drafted places, and when a later score
 // passes it by more than TT_ROOM powers of two, which the digits and the f16 range
-// have to spare (p = 1 keeps 23 bits).  Until then O gathers in TMEM over the
-// tiles, and a tile needs no maximum, no exchange and no rescaling.
+// have to spare (p = 1 keeps 23 bits).  Until then a tile needs no maximum, no
+// exchange and no rescaling, and O of an int8 cache gathers in TMEM.
 //
 // Roles (20 warps): 16 loads K and V tiles by TMA into a ring of slots, 17 issues
 // S = K . q^T (M = 128 positions), 18 issues O^T = V^T . p^T (M = dims; V is read
-// MN-major as it lies, p is written position by position), 19 finds the
-// next segment and prepares its columns, and four groups of four warps do the softmax, a thread per
-// position for S and a thread per dim for O, 16 columns at most.  The groups form
-// teams with a tile each: up to 16 columns four teams of one group, with 32 two
-// teams of two, with 64 one team of four, whose columns share one product.  (A
+// MN-major as it lies, p is written position by position), 19 finds the next
+// segment (and prepares its columns, up to 16), and four groups of four warps do
+// the softmax, a thread per position for S and a thread per dim for O, 16 columns
+// at most.  The groups form teams with a tile each: up to 16 columns four teams of
+// one group, with 32 two teams of two, with 64 one team of four, whose columns
+// share one product.  (A
 // product of few columns costs the 4 KB of its K or V rows, 40 cycles at 32
 // columns and 100 at 192: four of 48 took twice one of 192.)  The cache is so read
 // once for 64 columns.
+//
+// What bounds it, one B200.  Decode: the cache's bytes where it is long (64
+// sequences of 32000: f16 1162 us, 7.2 TB/s, int8 608 us, 7.1 TB/s with a head's
+// positions adjacent and 5.7 with 128-byte rows 1 KB apart), a share's start, its
+// units' ends and the joining where it is not (16 of up to 4095 int8 positions: 29
+// us, 3.1 TB/s; its SMs issue 29% of their cycles).  Wide trees: the softmax (24 trees
+// of 60 nodes over up to 6000: int8 421 us, f16 406; 64 columns keep 60% of the issue
+// slots and 21% of the tensor cores busy, 2.2 us a tile).
 constexpr int TT_GROUPS = 4, TT_SOFT = TT_GROUPS * 128, TT_THREADS = TT_SOFT + 128;
 constexpr int TT_TMA_WARP = 16, TT_S_WARP = 17, TT_O_WARP = 18, TT_NEXT_WARP = 19;
 constexpr int TT_TILE = 128;
@@ -143,8 +153,8 @@ constexpr float TT_DIGITS = 8355711.0f;  // 0x7f7f7f: the largest value of three
 constexpr float TT_ROOM = 6.0f;
 // Units of the p operand for p = 1 (with m < 2): 2^6 * 2 of them stay below 2^15 *
 // 0x7f7f, the largest value of its digits, 2^6 * 2^9 below f16's largest.
-// Room for 2^8 rescaled less often (24 trees of 60 nodes 594 us, 617 with 2^4) but
-// lost two digits' worth of the f32 sums' accuracy (1.5e-6 against 6e-7).
+// 2^4 sets references more often (24 trees of 60 nodes 447 us against 421); 2^8 lost
+// two digits' worth of the f32 sums' accuracy (1.5e-6 against 6e-7) for 1%.
 template <bool Q8>
 constexpr float TT_UNITS = Q8 ? 1069500000.0f / 128.0f : 512.0f;
 // Tiles that O may gather.  Digits: 2^21 x 512 fits 32 bits.  f32: none beyond
@@ -190,16 +200,16 @@ struct TtShape {
   // that time (600 KB of a 4096 context), and a kernel follows.
   static constexpr bool TICKET = CH <= 32;
   static_assert(TG * (CS + CO) <= 512, "TMEM");
-  // Warps that prepare the next segment's columns.  Up to 16, one warp does while
-  // the segment before ends (given to the softmax warps it made 24 sequences' decode 15%
-  // slower).  More are a chain of 8 or 16 trips to memory for that warp, which
-  // nothing hides (15 us for 64 columns): the softmax warps do them, one trip each
-  // (24 trees of 60 nodes 540 -> 485 us).
+  // Warps that prepare the next segment's columns.  Up to 16 columns one warp does, while
+  // the segment before ends (all softmax warps at its end: 24 sequences' decode 48.3
+  // us against 45.9).  More are a chain of 8 or 16 trips to memory for that warp, which
+  // nothing hides: the softmax warps do them, one trip each (24 trees of 60 nodes 421
+  // us against 538).
   static constexpr int STAGERS = CG == 1 ? 1 : TT_SOFT / 32;
-  // A segment's start and end, in tiles: 7 to 10 us against 2 of a wide tile, 3 against
-  // 0.9 of a decode tile.  (24 sequences of 6000, int8, are 2% slower with 2 and the
-  // same from 4 to 10; 24 trees of 60 nodes over 6000 f16 positions 495 us with 2, 462
-  // with 4, 434 with 8, but eight trees over 1000, int8, 70, 70 and 75.)
+  // A segment's start and end, in tiles.  2 / 4 / 8 of them: 24 sequences of up to
+  // 6000 int8 positions 47.9 / 45.9 / 45.1 us, 16 of 4095 f16 39.2 / 38.2 / 40.1; 24 trees
+  // of 60 nodes over 6000 f16 positions 419 / 406 / 376, eight over 1000 int8 61.3 /
+  // 60.7 / 66.5, where a long start leaves shares with little else.
   static constexpr int LEAD = 4;
   // tiles until V is in the same slot again; a group that waits for its V knows that
   // of its last tile has landed, and so all before
@@ -271,8 +281,8 @@ __device__ __forceinline__ F2 joined(const uint32_t* v, int c) {
 // once: the loops run on to their ends, so that named barriers stay matched.  A
 // try may suspend, for 20 us at most, since a spinning warp takes issue slots from
 // the rest; it takes 350 cycles even for a phase long over, a test 150, so that
-// comes first (three of them are slower again).  The loop stays
-// rolled: there are many waits, and the roles' loops lose 15% to instruction fetch.
+// comes first (three of them are slower again).  The loop stays rolled: there are
+// many waits, and unrolled ones cost the roles 20% in instruction fetch.
 constexpr uint32_t TT_POLLS = 1u << 17;
 __device__ __forceinline__ bool tt_wait(uint64_t* bar, uint32_t phase, volatile int* abort) {
   if (mbar_test_wait(bar, phase)) return true;
@@ -1272,8 +1282,9 @@ static size_t al256(size_t x) { return (x + 255) & ~(size_t)255; }
 // Columns of a CTA: as many as there are, up to 64, so that the cache is read
 // once.  33 to 64 of a few units are taken as two chunks of 32: with two tiles
 // or so for each SM, two teams and no merge kernel count for more than reading
-// twice (16 nodes x 4 heads over 4096 f16 positions, 8 kv heads: one sequence 29 us
-// against 36; four of 3000 46 against 43).
+// twice (16 nodes x 4 heads, 8 kv heads, f16: one sequence of 4096 positions 25.8 us
+// against 28.4, two of 3000 25.3 against 29.0, four 37.5 against 31.9; one of 30000, a
+// length that is not known here, 60 against 54).
 static int tt_columns(int max_nodes, int group, int units) {
   const int vh = max_nodes * group;
   return vh <= 8 ? 8 : vh <= 16 ? 16 : vh <= 32 || (vh <= 64 && units <= 16) ? 32 : 64;
