@@ -1203,14 +1203,14 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
         if (!whole) {
           if (S::TICKET) groups_sync();
           if (tid == 0) {
-            if (seg_no == 0) tt_wait(&parts0, 0, abort);
+            const bool known = seg_no || tt_wait(&parts0, 0, abort);
             const int i0 = seg_part[set].x, n = seg_part[set].y;
             if constexpr (S::TICKET) {
-              const bool last = ticket_acq_rel(ta.tickets + i0) == (unsigned)n - 1;
+              const bool last = known && ticket_acq_rel(ta.tickets + i0) == (unsigned)n - 1;
               if (last) ta.tickets[i0] = 0u;
               s_merge[0] = last ? n : 0;
               s_merge[1] = i0;
-            } else if (first_part) {
+            } else if (first_part && known) {
               ta.parts[blockIdx.x] = TreePart{n, cols, sg.vh0, sg.kvh, sg.off, {0, 0, 0}};
             }
           }
