@@ -38,7 +38,8 @@ __device__ __forceinline__ unsigned long long tree_mask(const TreeArgs& a, const
 }
 
 // Any head size and stride: one block per (node, head, sequence), 128
-// positions at a time; scores take a thread per position, P.V a thread per dim.
+// positions at a time; scores take a thread per position, P.V a thread per dim.  o is
+// kept divided by the sum, so that values near f32's largest do not pass it.
 constexpr int TR_THREADS = 128;
 
 template <bool Q8>
@@ -81,7 +82,9 @@ __global__ void __launch_bounds__(TR_THREADS) tree_simple_kernel(const TreeArgs 
     __syncthreads();
     float sum = 0.0f;
     for (int u = 0; u < TR_THREADS; u++) sum += p_s[u];
-    l = fmaf(l, alpha, sum);
+    const float before = l * alpha;
+    l = before + sum;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
     for (int e = 0; e < 2; e++) {
       const int d = tid + e * TR_THREADS;
@@ -92,14 +95,14 @@ __global__ void __launch_bounds__(TR_THREADS) tree_simple_kernel(const TreeArgs 
         const size_t row = (size_t)(s.start + t0 + u);
         float x = value(a.c.v, row * a.c.row_stride + (size_t)kvh * a.c.head_stride + d);
         if (Q8) x *= a.c.v_scale[row * a.c.scale_row + (size_t)kvh * a.c.scale_head];
-        acc = fmaf(p_s[u], x, acc);
+        acc = fmaf(p_s[u] * inv, x, acc);
       }
-      o[e] = fmaf(o[e], alpha, acc);
+      o[e] = fmaf(o[e], before * inv, acc);
     }
   }
 #pragma unroll
   for (int e = 0; e < 2; e++)
-    if (tid + e * TR_THREADS < hd) a.out[row_q + tid + e * TR_THREADS] = l == 0.0f ? 0.0f : o[e] / l;
+    if (tid + e * TR_THREADS < hd) a.out[row_q + tid + e * TR_THREADS] = o[e];
 }
 
 // ---------------------------------------------------------------- tcgen05
