@@ -122,7 +122,11 @@ __global__ void __launch_bounds__(TR_THREADS) tree_simple_kernel(const TreeArgs 
 // the score in f32.  The V scale, 2^e * m, goes with the probability: e is added to
 // the score (in powers of two), so that p * 2^e, what the place adds to the
 // output, is measured against a reference of the same kind, and m scales the
-// digits.
+// digits.  The sum of the probabilities takes p * 2^e * 2^-e.  With e within TT_SPAN
+// no weight that matters is lost on that way, a scale of 0 included (m = 0, any e).
+// A place whose scale lies beyond (or is no number) makes the sum NaN, and whose sum
+// is NaN in the end, tree_column computes from the definition, at a few us for every
+// 100 places.
 //   The reference of a column is its largest score when it was last set; it
 // is set at the first tile, at tiles with drafted places, and when a later score
 // passes it by more than TT_ROOM powers of two, which the digits and the f16 range
@@ -154,6 +158,7 @@ constexpr int TT_TILE = 128;
 constexpr int TT_MAX_SLOTS = 10;
 constexpr float TT_DIGITS = 8355711.0f;  // 0x7f7f7f: the largest value of three balanced digits
 constexpr float TT_ROOM = 6.0f;
+constexpr int TT_SPAN = 40;
 // Units of the p operand for p = 1 (with m < 2): 2^6 * 2 of them stay below 2^15 *
 // 0x7f7f, the largest value of its digits, 2^6 * 2^9 below f16's largest.
 // 2^4 sets references more often (24 trees of 60 nodes 447 us against 421); 2^8 lost
@@ -171,7 +176,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 // What a CTA leaves for tree_merge_kernel: the unit that began in it and went on
 // in the next n - 1 CTAs (n = 0: none).
 struct TreePart {
-  int n, cols, vh0, kvh, off, pad[3];
+  int n, cols, vh0, kvh, b, pad[3];
 };
 struct TreeTcArgs {
   CUtensorMap tm_k, tm_v;
@@ -395,6 +400,7 @@ struct TreeWalk {
 // What the softmax groups need of a segment; places count from its first tile.
 struct TreeSegment {
   int row, len, total, off;  // cache row of place 0; places all nodes see; places; first query row
+  int b;                     // sequence
   int kvh, tiles;
   int before, rest;          // the unit's tiles before and after this segment
   int vh0, cols;             // the chunk's first column of the unit, and its columns
@@ -428,6 +434,62 @@ __device__ __forceinline__ float tree_add(const TreeTcArgs& ta, int ch, int c, i
   }
   return warp_sum(sum);
 }
+// One column of an int8 cache from the definition, by a warp: for the few whose
+// places' V scales the digits do not take.  A place a lane for the scores, four dims
+// a lane for o, which is kept divided by the sum, so that values up to f32's
+// largest do not pass it.  (Rows start on 16 bytes and are made of them.)
+__device__ __noinline__ void tree_column(const TreeArgs& a, const TreeSeq& s, int kvh, int vh, int lane) {
+  const int group = a.n_heads / a.c.n_kv, node = vh / group, head = kvh * group + vh % group, hd = a.c.hd;
+  const size_t at = ((size_t)(s.off + node) * a.n_heads + head) * hd;
+  const float* q = a.q + at;
+  const unsigned long long mask = tree_mask(a, s, node);
+  const float scale = 1.0f / sqrtf((float)hd);
+  const int8_t *k8 = static_cast<const int8_t*>(a.c.k), *v8 = static_cast<const int8_t*>(a.c.v);
+  const size_t head_at = (size_t)kvh * a.c.head_stride, scale_at = (size_t)kvh * a.c.scale_head;
+  float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int t0 = 0; t0 < s.len + s.n; t0 += 32) {
+    const int t = t0 + lane;
+    const bool seen = t < s.len || (t < s.len + s.n && (mask >> (t - s.len) & 1));
+    float sc = -INFINITY;
+    if (seen) {
+      const size_t row = (size_t)(s.start + t);
+      const uint4* k = reinterpret_cast<const uint4*>(k8 + row * a.c.row_stride + head_at);
+      float dot = 0.0f;
+      for (int d = 0; d < hd; d += 16) {
+        const uint4 w = k[d / 16];
+        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int e = 0; e < 16; e++) dot = fmaf(q[d + e], (float)(int8_t)(ws[e / 4] >> (8 * (e % 4))), dot);
+      }
+      sc = dot * a.c.k_scale[row * a.c.scale_row + scale_at] * scale;
+    }
+    const float top = fmaxf(m, warp_max(sc)), ref = top == -INFINITY ? 0.0f : top;
+    float p = seen ? expf(sc - ref) : 0.0f;
+    const float before = l * expf(m - ref);
+    m = top;
+    l = before + warp_sum(p);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    p *= inv;
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (unsigned bits = __ballot_sync(0xffffffffu, seen); bits; bits &= bits - 1) {
+      const int u = __ffs((int)bits) - 1;
+      const float pu = __shfl_sync(0xffffffffu, p, u);
+      const size_t row = (size_t)(s.start + t0 + u);
+      const float vs = a.c.v_scale[row * a.c.scale_row + scale_at];
+      if (lane * 4 < hd) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(v8 + row * a.c.row_stride + head_at + lane * 4);
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[e] = fmaf(pu, (float)(int8_t)(w >> (8 * e)) * vs, acc[e]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) o[e] = fmaf(o[e], before * inv, acc[e]);
+  }
+  if (lane * 4 < hd) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) a.out[at + lane * 4 + e] = o[e];
+  }
+}
 // A ticket of a count over CTAs: what this CTA wrote (the others' writes ordered
 // before by the caller's barrier) is released, and the last to draw acquires it all.
 __device__ __forceinline__ unsigned ticket_acq_rel(unsigned* counter) {
@@ -438,7 +500,7 @@ __device__ __forceinline__ unsigned ticket_acq_rel(unsigned* counter) {
 
 __device__ __forceinline__ TreeSegment tree_segment(const TreeWalk& w) {
   const int skip = w.tile * TT_TILE, vh0 = w.chunk * w.ch;
-  return TreeSegment{w.s.start + skip, w.s.len - skip, w.s.len + w.s.n - skip, w.s.off, w.kvh, w.seg, w.tile,
+  return TreeSegment{w.s.start + skip, w.s.len - skip, w.s.len + w.s.n - skip, w.s.off, w.b, w.kvh, w.seg, w.tile,
                      w.tiles - w.tile - w.seg, vh0, min(w.ch, w.s.n * w.group - vh0), w.more()};
 }
 
@@ -471,6 +533,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
   __shared__ __align__(16) float x_m[16][NQ], x_d[16][NQ], x_al[16][NQ];
   __shared__ int x_on[4];                      // does a team's O go onto what its accumulator holds?
   __shared__ float2 x_fin[4][NQ];              // (max, sum) of a finished segment
+  __shared__ int s_nan;                        // a sum of a unit that is finished here is NaN
   __shared__ unsigned long long x_bad[4];   // drafted rows of V that are not finite
   __shared__ unsigned long long w_sum[TT_THREADS / 32], s_all;
   __shared__ int s_any;       // has the share a tile?
@@ -498,6 +561,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
     if (lane == 0) {
       s_abort = 0;
       s_any = 0;
+      s_nan = 0;
       any_mask[0] = any_mask[1] = 0ull;
       mbar_init(&q_ready, 32 * S::STAGERS);
       mbar_init(&q_free, 1);
@@ -932,15 +996,11 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
           const float vs = vs_next;
           if (t + TG < tiles) scales(t + TG);
           const uint32_t b = __float_as_uint(vs);
-          if (b >= 0x7f800000u) {  // negative, infinite or NaN: whoever sees the place gets NaN
-            ks = __int_as_float(0x7fffffff);
-          } else if (b < 0x00800000u) {
-            ve = -126;
-            vm = vs * 0x1p126f;
-          } else {
-            ve = (int)(b >> 23) - 127;
-            vm = __uint_as_float((b & 0x007fffffu) | 0x3f800000u);
-          }
+          ve = (int)(b >> 23) - 127;  // (a negative scale is beyond as well)
+          const bool in = (unsigned)(ve + TT_SPAN) <= 2 * TT_SPAN;
+          vm = in ? __uint_as_float((b & 0x007fffffu) | 0x3f800000u) : 0.0f;
+          if (!in) ve = -TT_SPAN;
+          if (!in && b) ks = __int_as_float(0x7fffffff);
         }
         // ---- scores (with V's exponent), in powers of two, against the references
         tt_wait(&s_full[tg], (uint32_t)item & 1, abort);
@@ -1035,13 +1095,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
         }
         // ---- probabilities, in the operand's form, a row per position
         if constexpr (Q8) {
-          const bool tiny = ve < -60;  // such a place's weight may be lost beside p * 2^ve: it is summed by itself
-          if (__any_sync(0xffffffffu, tiny)) {
-#pragma unroll
-            for (int c = 0; c < NQ; c += 2)
-              if (tiny) l[c / 2] = l[c / 2] + F2(ex2(s[c / 2].lo() - (float)ve), ex2(s[c / 2].hi() - (float)ve));
-          }
-          const F2 cm(vm * TT_UNITS<true>), iv(tiny ? 0.0f : __uint_as_float((uint32_t)(127 - ve) << 23));
+          const F2 cm(vm * TT_UNITS<true>), iv(__uint_as_float((uint32_t)(127 - ve) << 23));
           uint32_t dg[4][NQ / 4];
 #pragma unroll
           for (int c = 0; c < NQ; c += 4) {
@@ -1165,8 +1219,11 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
         for (int c = 0; c < NQ; c++) po[c * 128 + r] = c & 1 ? o[c / 2].hi() : o[c / 2].lo();
       }
       group_sync(g);
-      if (wq == 0 && lane < NQ)
-        x_fin[g][lane] = make_float2(ref, (x_sum[g][0][lane] + x_sum[g][1][lane]) + (x_sum[g][2][lane] + x_sum[g][3][lane]));
+      if (wq == 0 && lane < NQ) {
+        const float sum = (x_sum[g][0][lane] + x_sum[g][1][lane]) + (x_sum[g][2][lane] + x_sum[g][3][lane]);
+        x_fin[g][lane] = make_float2(ref, sum);
+        if (Q8 && sum != sum && !sg.before && !sg.rest) s_nan = 1;
+      }
       groups_sync();
       {
         const bool first_part = sg.before == 0, whole = first_part && !sg.rest;
@@ -1214,7 +1271,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
               s_merge[0] = last ? n : 0;
               s_merge[1] = i0;
             } else if (first_part && known) {
-              ta.parts[blockIdx.x] = TreePart{n, cols, sg.vh0, sg.kvh, sg.off, {0, 0, 0}};
+              ta.parts[blockIdx.x] = TreePart{n, cols, sg.vh0, sg.kvh, sg.b, {0, 0, 0}};
             }
           }
           if constexpr (S::TICKET) {
@@ -1239,7 +1296,9 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
                     for (int e = 0; e < 4; e++) x[e] += half[(wi + 1) * 128 + e * 32 + lane];
                   }
                 }
-                if (c < cols && wi % WPC == 0) {
+                if (Q8 && sum != sum) {
+                  if (wi % WPC == 0) tree_column(a, tree_seq(a, sg.b), sg.kvh, sg.vh0 + c, lane);
+                } else if (c < cols && wi % WPC == 0) {
 #pragma unroll
                   for (int e = 0; e < 4; e++)
                     if (e * 32 + lane < hd) out_seq[col_off[set][c] + e * 32 + lane] = sum == 0.0f ? 0.0f : x[e] / sum;
@@ -1251,6 +1310,15 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
       }
       more = sg.more;
       if (!Q8 && tid == 0) any_mask[set] = 0ull;
+      if (Q8 && s_nan) {
+        groups_sync();  // all have seen that, and the NaNs are written
+        for (int c = wi; c < sg.cols; c += TT_SOFT / 32) {
+          float sum = 0.0f;
+          for (int q = 0; q < TG; q++) sum += x_fin[q * CG + c / NQ][c % NQ].y;
+          if (sum != sum) tree_column(a, tree_seq(a, sg.b), sg.kvh, sg.vh0 + c, lane);
+        }
+        s_nan = 0;  // every warp meets before the next segment's end
+      }
       k0 += tiles;
       seg_no++;
     } while (more);
@@ -1274,8 +1342,13 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const __grid_constant__
   if (c >= ch || !u.n || c >= u.cols) return;
   float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   const float sum = tree_add<1>(ta, ch, c, i0, u.n, 0, lane, hd, x);
+  const TreeSeq s = tree_seq(a, u.b);
   const int vh = u.vh0 + c, node = vh / group, head = u.kvh * group + vh % group;
-  float* out = a.out + ((size_t)(u.off + node) * a.n_heads + head) * hd;
+  if (a.c.q8 && sum != sum) {
+    tree_column(a, s, u.kvh, vh, lane);
+    return;
+  }
+  float* out = a.out + ((size_t)(s.off + node) * a.n_heads + head) * hd;
 #pragma unroll
   for (int e = 0; e < 4; e++)
     if (e * 32 + lane < hd) out[e * 32 + lane] = sum == 0.0f ? 0.0f : x[e] / sum;
