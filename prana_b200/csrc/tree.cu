@@ -122,11 +122,11 @@ __global__ void __launch_bounds__(TR_THREADS) tree_simple_kernel(const TreeArgs 
 // the score in f32.  The V scale, 2^e * m, goes with the probability: e is added to
 // the score (in powers of two), so that p * 2^e, what the place adds to the
 // output, is measured against a reference of the same kind, and m scales the
-// digits.  The sum of the probabilities takes p * 2^e * 2^-e.  With e within TT_SPAN
-// no weight that matters is lost on that way, a scale of 0 included (m = 0, any e).
-// A place whose scale lies beyond (or is no number) makes the sum NaN, and whose sum
-// is NaN in the end, tree_column computes from the definition, at a few us for every
-// 100 places.
+// digits.  The sum of the probabilities takes p * 2^e * 2^-e.  With e from TT_E_MIN to
+// TT_E_MAX no weight that matters is lost on that way, a scale of 0 included (m = 0,
+// any e).  A place whose scale lies beyond (or is no number) makes the sum NaN, and a
+// column whose sum is NaN in the end, tree_column computes from the definition (8 us
+// for every 32 places).
 //   The reference of a column is its largest score when it was last set; it
 // is set at the first tile, at tiles with drafted places, and when a later score
 // passes it by more than TT_ROOM powers of two, which the digits and the f16 range
@@ -158,7 +158,9 @@ constexpr int TT_TILE = 128;
 constexpr int TT_MAX_SLOTS = 10;
 constexpr float TT_DIGITS = 8355711.0f;  // 0x7f7f7f: the largest value of three balanced digits
 constexpr float TT_ROOM = 6.0f;
-constexpr int TT_SPAN = 40;
+// V scales of 8.3e-25 to 1e6: the smallest weight beside the largest is 2^-100 by
+// these, and 2^-26 by the scores, in f32's range; and a sum stays below 2^(80 + 6) a place
+constexpr int TT_E_MIN = -80, TT_E_MAX = 20;
 // Units of the p operand for p = 1 (with m < 2): 2^6 * 2 of them stay below 2^15 *
 // 0x7f7f, the largest value of its digits, 2^6 * 2^9 below f16's largest.
 // 2^4 sets references more often (24 trees of 60 nodes 447 us against 421); 2^8 lost
@@ -450,9 +452,10 @@ __device__ __noinline__ void tree_column(const TreeArgs& a, const TreeSeq& s, in
   for (int t0 = 0; t0 < s.len + s.n; t0 += 32) {
     const int t = t0 + lane;
     const bool seen = t < s.len || (t < s.len + s.n && (mask >> (t - s.len) & 1));
-    float sc = -INFINITY;
+    float sc = -INFINITY, vs = 0.0f;
     if (seen) {
       const size_t row = (size_t)(s.start + t);
+      vs = a.c.v_scale[row * a.c.scale_row + scale_at];
       const uint4* k = reinterpret_cast<const uint4*>(k8 + row * a.c.row_stride + head_at);
       float dot = 0.0f;
       for (int d = 0; d < hd; d += 16) {
@@ -471,19 +474,26 @@ __device__ __noinline__ void tree_column(const TreeArgs& a, const TreeSeq& s, in
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     p *= inv;
     float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (unsigned bits = __ballot_sync(0xffffffffu, seen); bits; bits &= bits - 1) {
-      const int u = __ffs((int)bits) - 1;
-      const float pu = __shfl_sync(0xffffffffu, p, u);
-      const size_t row = (size_t)(s.start + t0 + u);
-      const float vs = a.c.v_scale[row * a.c.scale_row + scale_at];
-      if (lane * 4 < hd) {
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(v8 + row * a.c.row_stride + head_at + lane * 4);
+    const unsigned all = __ballot_sync(0xffffffffu, seen);
+#pragma unroll 1
+    for (int u0 = 0; u0 < 32; u0 += 8) {
+      uint32_t w[8];
 #pragma unroll
-        for (int e = 0; e < 4; e++) acc[e] = fmaf(pu, (float)(int8_t)(w >> (8 * e)) * vs, acc[e]);
+      for (int i = 0; i < 8; i++) {
+        const size_t row = (size_t)(s.start + t0 + u0 + i);
+        const bool take = lane * 4 < hd && (all >> (u0 + i) & 1);
+        w[i] = take ? *reinterpret_cast<const uint32_t*>(v8 + row * a.c.row_stride + head_at + lane * 4) : 0u;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const float pu = __shfl_sync(0xffffffffu, p, u0 + i), vu = __shfl_sync(0xffffffffu, vs, u0 + i);
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[e] = fmaf(pu, (float)(int8_t)(w[i] >> (8 * e)) * vu, acc[e]);
       }
     }
 #pragma unroll
     for (int e = 0; e < 4; e++) o[e] = fmaf(o[e], before * inv, acc[e]);
+    if (__all_sync(0xffffffffu, o[0] != o[0] && o[1] != o[1] && o[2] != o[2] && o[3] != o[3])) break;  // NaN from here on
   }
   if (lane * 4 < hd) {
 #pragma unroll
@@ -997,9 +1007,9 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
           if (t + TG < tiles) scales(t + TG);
           const uint32_t b = __float_as_uint(vs);
           ve = (int)(b >> 23) - 127;  // (a negative scale is beyond as well)
-          const bool in = (unsigned)(ve + TT_SPAN) <= 2 * TT_SPAN;
+          const bool in = (unsigned)(ve - TT_E_MIN) < TT_E_MAX - TT_E_MIN;
           vm = in ? __uint_as_float((b & 0x007fffffu) | 0x3f800000u) : 0.0f;
-          if (!in) ve = -TT_SPAN;
+          if (!in) ve = TT_E_MIN;
           if (!in && b) ks = __int_as_float(0x7fffffff);
         }
         // ---- scores (with V's exponent), in powers of two, against the references
