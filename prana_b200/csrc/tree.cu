@@ -1006,11 +1006,11 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
           const float vs = vs_next;
           if (t + TG < tiles) scales(t + TG);
           const uint32_t b = __float_as_uint(vs);
-          ve = (int)(b >> 23) - 127;  // (a negative scale is beyond as well)
+          ve = (int)(b >> 23 & 255u) - 127;
           const bool in = (unsigned)(ve - TT_E_MIN) < TT_E_MAX - TT_E_MIN;
-          vm = in ? __uint_as_float((b & 0x007fffffu) | 0x3f800000u) : 0.0f;
+          vm = in ? __uint_as_float((b & 0x807fffffu) | 0x3f800000u) : 0.0f;  // with its sign: the digits have theirs
           if (!in) ve = TT_E_MIN;
-          if (!in && b) ks = __int_as_float(0x7fffffff);
+          if (!in && vs != 0.0f) ks = __int_as_float(0x7fffffff);
         }
         // ---- scores (with V's exponent), in powers of two, against the references
         tt_wait(&s_full[tg], (uint32_t)item & 1, abort);

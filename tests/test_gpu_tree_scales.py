@@ -1,4 +1,4 @@
-"""attention_tree over int8 caches whose V scales are zero, tiny or huge.
+"""attention_tree over int8 caches whose V scales are zero, tiny, huge or negative.
 
 value = q * scale for any finite scale, so such a place takes part like another:
 its weight counts in the softmax's sum whatever its scale.  References and
@@ -117,4 +117,16 @@ def test_values_whose_weighted_sum_passes_f32(gpu, heads):
     for s in b.starts:  # int8 values of -1, 0 and 1, so that the values are finite
         b.cache.v[s + 5:s + 9].clamp_(-1, 1)
         b.cache.v_scale[s + 5:s + 9] = torch.tensor([2.0 ** 127, 2.0 ** 126, 3e38, 1e38], device="cuda")[:, None]
+    b.check()
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("q_scale", [0.5, 3.0])
+@pytest.mark.parametrize("length", [5, 700, 4000])
+def test_negative_scales(gpu, shape, q_scale, length):
+    b = batch(shape, length, q_scale)
+    for x in (b.cache.k_scale, b.cache.v_scale):
+        x[1::2] *= -1.0
+    for s in b.starts:
+        b.cache.v_scale[s + 2] = -0.0
     b.check()
