@@ -87,15 +87,18 @@ constexpr int WR_LANES = sizeof(T) == 2 ? 4 : 8;
 // round_clamp127(x * inv) of four values as bytes, from twice the quotients (a
 // power of two rounds alike): to the nearest with halves away from zero is
 // (n + 1) >> 1 of n = trunc(2 t) >= 0, and n >> 1 of n < 0; a NaN truncates to
-// 0.  |n| <= 254 by the scale itself, unless that is too small for f32: CLAMP.
-// The shifts are done on two 16-bit halves at once.
-template <bool CLAMP>
-__device__ __forceinline__ uint32_t quant_bytes(const float* x, float inv2) {
+// 0.  |n| <= 254 by the scale itself, and 2 inv is in f32's range, unless the scale
+// is tiny: SMALL doubles the quotient and clamps.  The shifts are done on two 16-bit
+// halves at once.
+template <bool SMALL>
+__device__ __forceinline__ uint32_t quant_bytes(const float* x, float inv) {
   uint32_t m[4];
+  const float f = SMALL ? inv : 2.0f * inv;
 #pragma unroll
   for (int e = 0; e < 4; e++) {
-    int n = __float2int_rz(__fmul_rn(x[e], inv2));
-    if (CLAMP) n = min(max(n, -254), 254);
+    const float t = __fmul_rn(x[e], f);
+    int n = __float2int_rz(SMALL ? 2.0f * t : t);
+    if (SMALL) n = min(max(n, -254), 254);
     m[e] = (uint32_t)(n + 1 + (n >> 31));
   }
   return __byte_perm(__byte_perm(m[0], m[1], 0x5410) >> 1, __byte_perm(m[2], m[3], 0x5410) >> 1, 0x6420);
@@ -146,7 +149,7 @@ __global__ void __launch_bounds__(RW_THREADS) kv_rows_write_wide(const KvRowsDev
 #pragma unroll
     for (int o = 1; o < LANES; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(mates, amax, o));
     const float scale = amax > 0.0f ? __fdiv_rn(amax, 127.0f) : 1.0f;
-    const float inv2 = 2.0f * __fdiv_rn(1.0f, scale);
+    const float inv = __fdiv_rn(1.0f, scale);
     int8_t* o = static_cast<int8_t*>(is_v ? c.v : c.k) + at;
 #pragma unroll
     for (int p = 0; p < PIECES; p++) {
@@ -154,7 +157,7 @@ __global__ void __launch_bounds__(RW_THREADS) kv_rows_write_wide(const KvRowsDev
       uint32_t w[E / 4];
 #pragma unroll
       for (int e = 0; e < E; e += 4)
-        w[e / 4] = scale < 1e-36f ? quant_bytes<true>(&f[p][e], inv2) : quant_bytes<false>(&f[p][e], inv2);
+        w[e / 4] = scale < 1e-36f ? quant_bytes<true>(&f[p][e], inv) : quant_bytes<false>(&f[p][e], inv);
       if (d < c.hd) {
         if constexpr (E == 8) *reinterpret_cast<uint2*>(o + d) = make_uint2(w[0], w[1]);
         else *reinterpret_cast<uint32_t*>(o + d) = w[0];
