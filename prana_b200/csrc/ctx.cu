@@ -635,7 +635,7 @@ int prana_kv_rows_write(prana_ctx* c, const prana_kv_rows* cache, const int32_t*
   NEED(src_type == PRANA_TYPE_F32 || src_type == PRANA_TYPE_F16, "source type %d is neither F32 nor F16", src_type);
   if (!n) return PRANA_OK;
   NEED(rows && k && v, "null argument");
-  NEED(n <= (size_t)INT32_MAX / d.n_kv, "%zu rows are too many", n);
+  NEED(n <= (size_t)(INT32_MAX - 1024) / d.n_kv, "%zu rows are too many", n);  // a last block's threads count on
   NEED(n == 1 || src_stride >= cache->n_kv_heads * cache->head_dim, "src_stride %zu is less than a row", src_stride);
   const size_t esz = src_type == PRANA_TYPE_F16 ? 2 : 4;
   NEED(aligned_to(k, esz) && aligned_to(v, esz) && aligned_to(rows, 4), "misaligned argument");
@@ -652,7 +652,7 @@ int prana_kv_rows_read(prana_ctx* c, const prana_kv_rows* cache, const int32_t* 
   NEED(dst_type == PRANA_TYPE_F32 || dst_type == PRANA_TYPE_F16, "destination type %d is neither F32 nor F16", dst_type);
   if (!n) return PRANA_OK;
   NEED(rows && k && v, "null argument");
-  NEED(n <= (size_t)INT32_MAX / d.n_kv, "%zu rows are too many", n);
+  NEED(n <= (size_t)(INT32_MAX - 1024) / d.n_kv, "%zu rows are too many", n);  // a last block's threads count on
   const size_t esz = dst_type == PRANA_TYPE_F16 ? 2 : 4;
   NEED(aligned_to(k, esz) && aligned_to(v, esz) && aligned_to(rows, 4), "misaligned argument");
   DevScope ds(c->device);
