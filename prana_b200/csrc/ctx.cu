@@ -695,7 +695,8 @@ int prana_attention_tree(prana_ctx* c, const float* q, const prana_kv_rows* cach
   NEED(n_heads > 0 && n_heads <= 65535 && n_heads % cache->n_kv_heads == 0, "n_heads must be a multiple of n_kv_heads");
   NEED(n_heads / cache->n_kv_heads <= 1024, "more than 1024 heads share a kv head");
   NEED(max_nodes <= (size_t)TREE_MAX_NODES, "%zu nodes per sequence exceed %d", max_nodes, TREE_MAX_NODES);
-  if (!n_seq || !n_nodes || !max_nodes) return PRANA_OK;
+  if (!n_seq || !n_nodes) return PRANA_OK;
+  NEED(max_nodes > 0, "max_nodes is 0, yet there are %zu nodes", n_nodes);
   NEED(q && starts && lens && node_offsets && out, "null argument");
   NEED(n_seq <= (size_t)INT32_MAX && n_nodes <= (size_t)INT32_MAX, "too many sequences or nodes");
   NEED(aligned_to(q, 4) && aligned_to(out, 4) && aligned_to(starts, 4) && aligned_to(lens, 4) &&
