@@ -241,7 +241,8 @@ int prana_kv_rows_move(prana_ctx *ctx, const prana_kv_rows *cache, const int32_t
  * included); masks NULL: node i sees nodes 0..i (a chain: attention_verify,
  * attention.rs:296-333, for many sequences; with one node each,
  * attention_decode, attention.rs:129-160).  Scores are scaled by 1/sqrt(head_dim);
- * a node that sees nothing gets zeros; what a node does not see has no effect
+ * a node that sees nothing gets zeros; rows of out that belong to no sequence, or to
+ * one that does not fit, stay as they are; what a node does not see has no effect
  * on it, NaN included, while a NaN or infinity in what it does see may make its
  * row NaN.
  * workspace: NULL for the context's scratch (then calls on several streams must

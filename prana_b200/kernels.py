@@ -462,7 +462,9 @@ def attention_tree(q: torch.Tensor, cache: KvRows, starts: torch.Tensor, lens: t
     j's K / V in row starts[b] + lens[b] + j.  Every node sees its context and the
     nodes whose bits are set in its mask (int64 [n_nodes], see tree_masks; None:
     itself and the nodes before it).  With one node per sequence this is
-    attention_decode for a batch.  starts, lens, offsets are int32."""
+    attention_decode for a batch.  starts, lens, offsets are int32.  A row that no
+    sequence fills (one past offsets[n_seq], or of a sequence that does not fit) stays
+    as it is in `out`, and is undefined in a result that this call allocates."""
     n_seq, n_nodes, device = starts.numel(), q.shape[0], cache.device
     width = n_heads * cache.head_dim
     if q.dtype != torch.float32 or q.device != device or not q.is_contiguous() or q.numel() != n_nodes * width:
