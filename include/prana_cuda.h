@@ -216,7 +216,9 @@ typedef struct prana_kv_rows {
 } prana_kv_rows;
 /* Row rows[i] of the cache = row i of k and v ([n, n_kv_heads * head_dim], F32 or
  * F16, src_stride elements from row to row), for rows[i] >= 0 (a negative index
- * skips the row; an index named twice gets one of its rows).  An int8 cache
+ * skips the row).  The others must differ: a cache row named twice ends up as any
+ * mixture of its sources, an int8 one's scale and values of different rows among
+ * them.  An int8 cache
  * quantises each head row as quantize_q8 does a block (matmul.rs:61-84): scale =
  * amax / 127 (1 when amax is 0), round half away from zero, NaN to 0; a row
  * holding an infinity gets an infinite scale and reads back as NaN.  An f16

@@ -400,7 +400,8 @@ class KvRows:
 
 def kv_rows_write(cache: KvRows, rows: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
     """Cache row rows[i] (int32; negative: skipped) = row i of k and v, [n, n_kv_heads,
-    head_dim] or [n, n_kv_heads * head_dim] in float32 or float16.  An int8 cache
+    head_dim] or [n, n_kv_heads * head_dim] in float32 or float16.  The indexes of 0 and
+    up must differ: a row named twice holds any mixture of its sources.  An int8 cache
     quantises each head row as it is written: scale = amax / 127, as quantize_q8."""
     n, device = rows.numel(), cache.device
     width = cache.n_kv_heads * cache.head_dim
