@@ -358,8 +358,7 @@ static cudaError_t write_go(const KvRowsDev& c, const int* rows, const T* k, con
     case 1: return GO(1);
     case 2: return GO(2);
     case 4: return GO(4);
-    case 8: return GO(8);
-    default: return GO(16);
+    default: return GO(8);
   }
 #undef GO
 }
