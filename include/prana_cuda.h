@@ -203,7 +203,9 @@ int prana_attention(prana_ctx *ctx, const float *q, const float *k, const float 
  * head's positions are adjacent (row_stride = head_dim).  Row indexes, starts,
  * lengths, paths and masks are DEVICE arrays.  What they hold is checked on the
  * device: a row or a sequence that does not fit is left out, and the next
- * prana_ctx_synchronize returns PRANA_E_INVALID, once.  Calls never synchronize. */
+ * prana_ctx_synchronize returns PRANA_E_INVALID, once.  Calls do not
+ * synchronize, but for prana_attention_tree without a workspace when the
+ * context's scratch has to grow. */
 #define PRANA_KV_F16 0
 #define PRANA_KV_Q8 1
 typedef struct prana_kv_rows {
@@ -248,7 +250,7 @@ int prana_kv_rows_move(prana_ctx *ctx, const prana_kv_rows *cache, const int32_t
  * on it, NaN included, while a NaN or infinity in what it does see may make its
  * row NaN.
  * workspace: NULL for the context's scratch (then calls on several streams must
- * not overlap), or workspace_bytes of 256-byte aligned device memory, at least
+ * not overlap, and one that needs more of it than any before waits for the stream), or workspace_bytes of 256-byte aligned device memory, at least
  * what prana_attention_tree_workspace says, not shared by overlapping calls.
  * Zero its first 4096 bytes before its first use (and after PRANA_E_TIMEOUT):
  * every call finds counters there at zero and leaves them so.  With a workspace
