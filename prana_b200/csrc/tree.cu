@@ -921,8 +921,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
       float ks_next = 0.0f, vs_next = 0.0f;
       auto scales = [&](int t) {  // of tile t's place r, and on to the group's next tile
         const bool in = t * TT_TILE + r < total;
-        ks_next = in ? __ldg(ks_at) : 0.0f;
-        vs_next = in ? __ldg(vs_at) : 0.0f;
+        ks_next = in ? *ks_at : 0.0f;
+        vs_next = in ? *vs_at : 0.0f;
         ks_at += (size_t)(TG * TT_TILE) * a.c.scale_row;
         vs_at += (size_t)(TG * TT_TILE) * a.c.scale_row;
       };
