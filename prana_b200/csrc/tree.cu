@@ -7,6 +7,7 @@
 // A place that a node does not see takes no part, whatever it holds.
 #include <atomic>
 #include <climits>
+#include <type_traits>
 
 #include "internal.h"
 #include "mbar.cuh"
@@ -132,6 +133,16 @@ __global__ void __launch_bounds__(TR_THREADS) tree_simple_kernel(const TreeArgs 
 // passes it by more than TT_ROOM powers of two, which the digits and the f16 range
 // have to spare (p = 1 keeps 23 bits).  Until then a tile needs no maximum, no
 // exchange and no rescaling, and O of an int8 cache gathers in TMEM.
+//   The digits' unit is 2^-23 of p = 1, and a long context may hold many places below
+// half of that.  So the references of an int8 cache come down as well: they are set
+// again after a tile that began them or raised one by TT_FAR (whose own digits use
+// TT_SPARE of the room, which no later tile needs), and after every RUN tiles; where
+// the largest score is then TT_LOW lower, to TT_ABOVE above it.  l goes to the
+// columns' sums at the same times, since a thread's own sum would round small
+// weights away.  (One score 18 above 16384 others, 64 columns: the error is 3e-6 of the
+// large value with references that only rise, 4e-7 so.  24 trees of 60 nodes 423 and
+// 450 us, 16 sequences' decode 31.8 and 32.3; a reference at each tile's largest score: 520
+// us and 33.)
 //
 // Roles (20 warps): 16 loads K and V tiles by TMA into a ring of slots, 17 issues
 // S = K . q^T (M = 128 positions), 18 issues O^T = V^T . p^T (M = dims; V is read
@@ -167,12 +178,11 @@ constexpr int TT_E_MIN = -80, TT_E_MAX = 20;
 // two digits' worth of the f32 sums' accuracy (1.5e-6 against 6e-7) for 1%.
 template <bool Q8>
 constexpr float TT_UNITS = Q8 ? 1069500000.0f / 128.0f : 512.0f;
-// Tiles that O may gather.  Digits: 2^21 x 512 fits 32 bits.  f32: none beyond
-// the tile, since the tensor core cuts sums off where it does not round them
-// (66000 positions: an error of 4.8e-6 with 31 tiles, 2.0e-6 with four, 6.5e-7 with
-// one, at no cost in time).
-template <bool Q8>
-constexpr int TT_RUN = Q8 ? 512 : 1;
+// How far below its reference a column's largest score brings it down, and to what above the score
+constexpr float TT_LOW = 8.0f, TT_ABOVE = 4.0f;
+constexpr float TT_FAR = 12.0f;    // a rise after which the next tile sets the references again
+constexpr float TT_SPARE = 5.0f;   // a power of two is left for the rounding of the scores
+constexpr float TT_DEPTH = 24.0f;  // further below a column's largest score no reference goes: f32 sums do not show it
 constexpr float LOG2E = 1.4426950408889634f;
 
 // What a CTA leaves for tree_merge_kernel: the unit that began in it and went on
@@ -209,6 +219,12 @@ struct TtShape {
   // and its two waits (4 us of a call); 64 columns are more than one SM reads in
   // that time (600 KB of a 4096 context), and a kernel follows.
   static constexpr bool TICKET = CH <= 32;
+  // Tiles of a team until an int8 cache's references are set in any case (O, which gathers
+  // until then, has 2^21 a tile at most).  An f16 cache's are not: its p reaches down to 2^-33 of
+  // the reference.  And its O gathers one tile, since the tensor core cuts sums off where
+  // it does not round them (66000 positions: an error of 4.8e-6 with 31 tiles, 2.0e-6
+  // with four, 6.5e-7 with one, at no cost in time).
+  static constexpr int RUN = CG == 4 ? 16 : 8;
   static_assert(TG * (CS + CO) <= 512, "TMEM");
   // Warps that prepare the next segment's columns.  Up to 16 columns one warp does, while
   // the segment before ends (all softmax warps at its end: 24 sequences' decode 48.3
@@ -538,9 +554,10 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
   __shared__ unsigned long long col_mask[2][CH], any_mask[2];
   __shared__ int col_off[2][CH];
   __shared__ __align__(16) float col_mul[2][CH];
-  __shared__ __align__(16) float x_max[4][4][NQ], x_sum[4][4][NQ];
+  __shared__ __align__(16) float x_max[4][4][NQ];
   // per warp: minus a column's reference, minus its last rise, what that does to l and o
   __shared__ __align__(16) float x_m[16][NQ], x_d[16][NQ], x_al[16][NQ];
+  __shared__ float4 x_col[16][NQ];             // per warp: a column's reference, its largest score, the sum so far and what that rounded away
   __shared__ int x_on[4];                      // does a team's O go onto what its accumulator holds?
   __shared__ float2 x_fin[4][NQ];              // (max, sum) of a finished segment
   __shared__ int s_nan;                        // a sum of a unit that is finished here is NaN
@@ -938,13 +955,49 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
         if (S::STAGERS > 1) mbar_arrive(&q_ready);
       }
       F2 l[NQ / 2], o[NQ / 2];
-      float ref = -INFINITY;  // lane c: the reference of column c; none yet
-      int run = 0;            // tiles against the present references
+      if (lane < NQ) x_col[wi][lane] = make_float4(-INFINITY, -INFINITY, 0.0f, 0.0f);
+      int left = 0;           // tiles until the references are due
       bool held = false;      // O holds tiles that are not in o
 #pragma unroll
       for (int c = 0; c < NQ / 2; c++) l[c] = o[c] = F2(0.0f);
       if (!Q8 && r == 0) x_bad[g] = 0ull;
 
+      // l, summed over the warp, joins the columns' sums
+      auto sums = [&]() {
+        float v[NQ];
+#pragma unroll
+        for (int c = 0; c < NQ / 2; c++) {
+          v[2 * c] = l[c].lo();
+          v[2 * c + 1] = l[c].hi();
+          l[c] = F2(0.0f);
+        }
+        auto halve = [&](auto columns, int bit) {  // a lane keeps half of its columns, and the other's of the same
+          constexpr int n = decltype(columns)::value;
+          const bool upper = lane & bit;
+#pragma unroll
+          for (int i = 0; i < n; i++) {
+            const float other = __shfl_xor_sync(0xffffffffu, upper ? v[i] : v[i + n], bit);
+            v[i] = (upper ? v[i + n] : v[i]) + other;
+          }
+        };
+        if constexpr (NQ == 16) halve(std::integral_constant<int, 8>(), 16);
+        halve(std::integral_constant<int, 4>(), 128 / NQ);
+        halve(std::integral_constant<int, 2>(), 64 / NQ);
+        halve(std::integral_constant<int, 1>(), 32 / NQ);
+        if constexpr (NQ == 8) v[0] += __shfl_xor_sync(0xffffffffu, v[0], 2);
+        v[0] += __shfl_xor_sync(0xffffffffu, v[0], 1);
+        __syncwarp();
+        if (lane % (32 / NQ) == 0) {
+          float4& at = x_col[wi][lane / (32 / NQ)];
+          if (Q8) {  // and what that rounds away
+            const float sum = at.z + v[0], part = sum - at.z;
+            at.w += (at.z - (sum - part)) + (v[0] - part);
+            at.z = sum;
+          } else {
+            at.z += v[0];
+          }
+        }
+      };
       // O into the registers
       auto fold = [&]() {
         tt_wait(&o_full[tg], (uint32_t)(item - 1) & 1, abort);
@@ -978,6 +1031,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
       };
 
       for (int t = first; t < tiles; t += TG, item++) {
+        // (not where drafted places are: what one node sees must not change the order of another's sum)
+        if (Q8 && left == 0 && t != first && (!trees || (t + 1) * TT_TILE <= len)) sums();
         const int pos = t * TT_TILE + r, j = pos - len;
         const bool edge = (t + 1) * TT_TILE > len;  // drafted places or none at all among the tile's
         const bool there = pos < total;
@@ -1051,8 +1106,9 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
         }
         // tiles with drafted places set the references anew each: whether another
         // node's score passes its reference must not touch this one's sums
-        bool fresh = run == 0 || (edge && trees);
-        if (run) {
+        const bool due = left == 0;  // (an f16 cache: at the first tile)
+        bool fresh = due || (edge && trees);
+        if (t != first) {
           float top = -INFINITY;
 #pragma unroll
           for (int c = 0; c < NQ; c += 4) {
@@ -1063,12 +1119,12 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
           }
           if (!fresh) fresh = team_any<CG>(tg, top > TT_ROOM);
         }
-        if (held && (fresh || run % TT_RUN<Q8> == 0)) {
+        if (held && (fresh || !Q8)) {
           fold();
           held = false;
         }
         if (fresh) {
-          // ---- the references: a column's largest score so far
+          // ---- the references
 #pragma unroll
           for (int c = 0; c < NQ; c += 4) {
             float4 m;
@@ -1079,18 +1135,40 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
             if (lane == 0) *reinterpret_cast<float4*>(&x_max[g][wq][c]) = m;
           }
           group_sync(g);
+          bool soon = false;
           if (lane < NQ) {
             // against the old reference, or against 0 where there is none
             const float m = fmaxf(fmaxf(x_max[g][0][lane], x_max[g][1][lane]), fmaxf(x_max[g][2][lane], x_max[g][3][lane]));
-            const bool none = ref == -INFINITY;
-            const float up = none ? (m == -INFINITY ? 0.0f : m) : fmaxf(m, 0.0f);
-            x_al[wi][lane] = none ? 1.0f : ex2(-up);
-            if (!none) ref += up;
-            else if (m != -INFINITY) ref = m;
-            x_m[wi][lane] = ref == -INFINITY ? 0.0f : -ref;
+            float4 at = x_col[wi][lane];
+            const bool none = at.x == -INFINITY;
+            float up = none ? (m == -INFINITY ? 0.0f : m) : fmaxf(m, 0.0f);
+            const float top = none ? m : at.x + m;  // the tile's largest score
+            soon = none || top - at.y > TT_FAR;
+            if (Q8 && !none) {
+              // whole powers of two, so that rescaling rounds nothing
+              if (m < -TT_LOW && m != -INFINITY) up = fmaxf(m + TT_ABOVE, at.y - TT_DEPTH - at.x);
+              up = ceilf(up);
+            }
+            if (Q8 && soon && fabsf(top) < 65536.0f) up -= TT_SPARE;
+            const float al = none ? 1.0f : ex2(-up);
+            if (!none) at.x += up;
+            else if (m != -INFINITY) at.x = up;
+            at.y = fmaxf(at.y, top);
+            at.z *= al;
+            at.w *= al;
+            x_col[wi][lane] = at;
+            x_al[wi][lane] = al;
+            x_m[wi][lane] = at.x == -INFINITY ? 0.0f : -at.x;
             x_d[wi][lane] = -up;
           }
-          group_sync(g);  // the tables are written, and x_max may be again
+          // the tables are written, and x_max may be again
+          if constexpr (Q8) {
+            soon = team_any<CG>(tg, soon);
+            left = soon ? 1 : due ? S::RUN : left;
+          } else {
+            group_sync(g);
+            left = 1;
+          }
 #pragma unroll
           for (int c = 0; c < NQ; c += 4) {
             const float4 m = *reinterpret_cast<const float4*>(&x_d[wi][c]), al = *reinterpret_cast<const float4*>(&x_al[wi][c]);
@@ -1101,7 +1179,6 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
             o[c / 2] = o[c / 2] * F2(al.x, al.y);
             o[c / 2 + 1] = o[c / 2 + 1] * F2(al.z, al.w);
           }
-          run = 0;
         }
         // ---- probabilities, in the operand's form, a row per position
         if constexpr (Q8) {
@@ -1184,7 +1261,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
         }
         if (r == 0 && cg == 0) x_on[tg] = held;
         held = true;
-        run++;
+        if (Q8) left--;
         fence_async_smem();
         mbar_arrive(&p_full[tg]);
       }
@@ -1217,12 +1294,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
       }
 
       // ---- the segment's (max, sum, o): the groups of a column range meet through their idle p operands
-#pragma unroll
-      for (int c = 0; c < NQ; c += 4) {
-        const float4 x = make_float4(warp_sum(l[c / 2].lo()), warp_sum(l[c / 2].hi()), warp_sum(l[c / 2 + 1].lo()),
-                                     warp_sum(l[c / 2 + 1].hi()));
-        if (lane == 0) *reinterpret_cast<float4*>(&x_sum[g][wq][c]) = x;
-      }
+      sums();
       if constexpr (TG > 1) {
         float* po = reinterpret_cast<float*>(p_t) + cg * NQ * 128;
 #pragma unroll
@@ -1230,8 +1302,9 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const __grid_con
       }
       group_sync(g);
       if (wq == 0 && lane < NQ) {
-        const float sum = (x_sum[g][0][lane] + x_sum[g][1][lane]) + (x_sum[g][2][lane] + x_sum[g][3][lane]);
-        x_fin[g][lane] = make_float2(ref, sum);
+        const float sum = (x_col[wi][lane].z + x_col[wi + 1][lane].z) + (x_col[wi + 2][lane].z + x_col[wi + 3][lane].z) +
+                          (Q8 ? (x_col[wi][lane].w + x_col[wi + 1][lane].w) + (x_col[wi + 2][lane].w + x_col[wi + 3][lane].w) : 0.0f);
+        x_fin[g][lane] = make_float2(x_col[wi][lane].x, sum);
         if (Q8 && sum != sum && !sg.before && !sg.rest) s_nan = 1;
       }
       groups_sync();
