@@ -198,7 +198,9 @@ int prana_attention(prana_ctx *ctx, const float *q, const float *k, const float 
  * memory the caller owns: [positions, n_kv_heads, head_dim] with the given
  * element strides (the last dimension is contiguous), as f16 or as int8 with
  * one f32 scale per position and head, [positions, n_kv_heads] with strides of
- * its own: value = q * scale.  head_dim is at most 256.  One such cache may hold
+ * its own: value = q * scale, for any finite scale (attention takes V scales of 0
+ * and 2^-80 to 2^20, of either sign, fast, and others by a slow form).  head_dim is
+ * at most 256.  One such cache may hold
  * the rows of many sequences; attention streams int8 rows fastest where one
  * head's positions are adjacent (row_stride = head_dim).  Row indexes, starts,
  * lengths, paths and masks are DEVICE arrays.  What they hold is checked on the

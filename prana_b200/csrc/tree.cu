@@ -157,12 +157,12 @@ __global__ void __launch_bounds__(TR_THREADS) tree_simple_kernel(const TreeArgs 
 // once for 64 columns.
 //
 // What bounds it, one B200.  Decode: the cache's bytes where it is long (64
-// sequences of 32000: f16 1162 us, 7.2 TB/s, int8 608 us, 7.1 TB/s with a head's
-// positions adjacent and 5.7 with 128-byte rows 1 KB apart), a share's start, its
-// units' ends and the joining where it is not (16 of up to 4095 int8 positions: 29
-// us, 3.1 TB/s; its SMs issue 29% of their cycles).  Wide trees: the softmax (24 trees
-// of 60 nodes over up to 6000: int8 421 us, f16 406; 64 columns keep 60% of the issue
-// slots and 21% of the tensor cores busy, 2.2 us a tile).
+// sequences of 32000: f16 1153 us, 7.3 TB/s, int8 618 us, 7.0 TB/s with a head's
+// positions adjacent and 6.0 with 128-byte rows 1 KB apart), a share's start, its
+// units' ends and the joining where it is not (16 of up to 4095 int8 positions: 32
+// us, 2.8 TB/s; its SMs issue 28% of their cycles).  Wide trees: the softmax (24 trees
+// of 60 nodes over up to 6000: int8 450 us, f16 440; 64 columns keep 65% of the issue
+// slots and 20% of the tensor cores busy).
 constexpr int TT_GROUPS = 4, TT_SOFT = TT_GROUPS * 128, TT_THREADS = TT_SOFT + 128;
 constexpr int TT_TMA_WARP = 16, TT_S_WARP = 17, TT_O_WARP = 18, TT_NEXT_WARP = 19;
 constexpr int TT_TILE = 128;
@@ -174,8 +174,8 @@ constexpr float TT_ROOM = 6.0f;
 constexpr int TT_E_MIN = -80, TT_E_MAX = 20;
 // Units of the p operand for p = 1 (with m < 2): 2^6 * 2 of them stay below 2^15 *
 // 0x7f7f, the largest value of its digits, 2^6 * 2^9 below f16's largest.
-// 2^4 sets references more often (24 trees of 60 nodes 447 us against 421); 2^8 lost
-// two digits' worth of the f32 sums' accuracy (1.5e-6 against 6e-7) for 1%.
+// With references that only rose, a room of 2^4 set them more often (24 trees of 60 nodes 447
+// us against 421), and 2^8 took accuracy (an error of 1.5e-6 against 6e-7) for 1%.
 template <bool Q8>
 constexpr float TT_UNITS = Q8 ? 1069500000.0f / 128.0f : 512.0f;
 // How far below its reference a column's largest score brings it down, and to what above the score

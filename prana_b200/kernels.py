@@ -54,8 +54,9 @@ def quantize_q8(rows: int, cols: int, w) -> tuple[np.ndarray, np.ndarray]:
 
 
 def synchronize(device: int | None = None) -> None:
-    """Wait for this device's kernel-level calls; raises PranaError
-    (PRANA_E_TIMEOUT) when a bounded device wait gave up in one of them."""
+    """Wait for this device's kernel-level calls; raises PranaError when a bounded
+    device wait gave up in one of them (PRANA_E_TIMEOUT), or when one was given rows
+    or lengths outside its cache (PRANA_E_INVALID)."""
     try:
         call("prana_ctx_synchronize", context(device))
     except _ffi.PranaError:
@@ -334,9 +335,9 @@ _SRC_TYPES = {torch.float32: TYPE_F32, torch.float16: TYPE_F16}
 class KvRows:
     """One layer's K and V rows [positions, n_kv_heads, head_dim] in torch CUDA
     memory: float16, or int8 with f32 scales [positions, n_kv_heads] (value =
-    q * scale).  Any strides, as long as the last dimension is contiguous and k
-    and v (and the two scales) are laid out alike.  The rows of many sequences
-    may share one KvRows."""
+    q * scale; attention is fast at V scales of 0 and 2^-80 to 2^20, of either sign).
+    Any strides, as long as the last dimension is contiguous and k and v (and the two
+    scales) are laid out alike.  The rows of many sequences may share one KvRows."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "quantized", "device", "n_kv_heads", "head_dim", "_view", "_ref")
 
@@ -379,7 +380,7 @@ class KvRows:
               device: int | str | torch.device = "cuda") -> "KvRows":
         """A zeroed cache.  Rows and scales lie head by head, so that one head's
         positions are adjacent: attention over 64 sequences of 32000 int8 positions
-        takes 608 us so and 753 position by position (f16 1162 and 1189); writing
+        takes 618 us so and 723 position by position (f16 1153 and 1205); writing
         and reading rows costs the same, up to 8% more where rows are scattered."""
         shape, dt = (n_kv_heads, positions, head_dim), torch.int8 if quantized else torch.float16
         k, v = (torch.zeros(shape, dtype=dt, device=device).transpose(0, 1) for _ in range(2))
