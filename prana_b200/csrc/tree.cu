@@ -125,7 +125,8 @@ __global__ void __launch_bounds__(TR_THREADS) tree_simple_kernel(const TreeArgs 
 // output, is measured against a reference of the same kind, and m scales the
 // digits.  The sum of the probabilities takes p * 2^e * 2^-e.  With e from TT_E_MIN to
 // TT_E_MAX no weight that matters is lost on that way, a scale of 0 included (m = 0,
-// any e).  A place whose scale lies beyond (or is no number) makes the sum NaN, and a
+// e = TT_E_MIN: only where such places outweigh the rest 2^80 times, what is left of the
+// rest is cut to 0).  A place whose scale lies beyond (or is no number) makes the sum NaN, and a
 // column whose sum is NaN in the end, tree_column computes from the definition (8 us
 // for every 32 places).
 //   The reference of a column is its largest score when it was last set; it
